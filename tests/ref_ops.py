@@ -28,7 +28,8 @@ def _f(x):
 # replaced by id 0 and a bit is raised; the step's results are then void.
 STATUS_BITS = {1: "a bounded wait inside a kernel ran out", 2: "a token id outside the vocabulary",
                4: "a block-table entry outside the page pool", 8: "a state slot outside the slots",
-               16: "a position outside its request's block-table row"}
+               16: "a position outside its request's block-table row", 32: "spans of more rows than the step has, or a row outside it",
+               64: "a drafted row whose parent is not before it, or a tree of too many rows"}
 _status = torch.zeros(1, dtype=torch.int32)
 
 
@@ -749,3 +750,142 @@ def mlstm(y, at, bias_i, bias_f, cap, norm_w, eps, state, step, heads, dim, vdim
     o = out * torch.rsqrt((out * out).mean(-1, keepdim=True) + eps)
     g = torch.sigmoid(_f(y[:, g_at:g_at + H * Dv]))
     return (o.reshape(N, H * Dv) * _f(norm_w) * g).to(y.dtype)
+
+
+# ---- steps that check drafted tokens: loops over requests and rows, in 64 bits
+def token_logprobs(logits, tokens, top=0):
+    x = logits.double()
+    p = torch.log_softmax(x, dim=1)
+    R, V = x.shape
+    asked = (tokens >= 0) & (tokens < V)
+    if bool(((tokens < -1) | (tokens >= V)).any()):
+        _raise(2)
+    t = torch.where(asked, tokens, torch.zeros_like(tokens)).long()[:, None]
+    xt, j = x.gather(1, t), torch.arange(V, device=x.device)
+    rank = ((x > xt) | ((x == xt) & (j < t))).sum(1).int()
+    weighted = torch.where(p == float("-inf"), torch.zeros_like(p), p.exp() * p)
+    order = torch.sort(x, dim=1, descending=True, stable=True).indices[:, :top]
+    lp = p.gather(1, t)[:, 0]
+    from zig_ai_b200.kernels.ops import TokenLogprobs
+    return TokenLogprobs(torch.where(asked, lp, torch.zeros_like(lp)), -weighted.sum(1), torch.where(asked, rank, torch.full_like(rank, -1)),
+                         order.int(), p.gather(1, order))
+
+
+def step_layout(q_lens, ctx_lens, slots, page_rows, page_size, n_rows, width, parents=None, tree_rows=0):
+    from zig_ai_b200.kernels.ops import StepLayout
+    dev, N, S = q_lens.device, int(n_rows), q_lens.numel()
+    cu, pos, seq, kv, tables, mask = [0], [], [], [], [], []
+    words = (tree_rows + 31) // 32 if parents is not None else 0
+    for s in range(S):
+        n, c = max(int(q_lens[s]), 0), max(int(ctx_lens[s]), 0)
+        if int(q_lens[s]) < 0 or cu[-1] + n > N:
+            _raise(32)
+        if int(ctx_lens[s]) < 0:
+            _raise(16)
+        n = min(n, N - cu[-1])
+        slot = int(_checked(slots[s:s + 1], page_rows.shape[0], 8))
+        row = [int(p) for p in page_rows[slot, :width]] + [0] * (width - page_rows.shape[1])
+        tables.append(row)
+        up = [] if parents is None else [int(p) for p in parents[cu[-1]:cu[-1] + n]]
+        for i in range(n):
+            at = (c + i) // page_size
+            seq.append(s)
+            if at >= min(width, page_rows.shape[1]):
+                _raise(16)
+                kv.append(-1)
+            elif row[at] < 0:
+                _raise(4)
+                kv.append(-1)
+            else:
+                kv.append(row[at] * page_size + (c + i) % page_size)
+            bits, depth = 0, i
+            if words and i >= tree_rows:
+                _raise(64)
+            elif words:
+                bits, cur, depth = 1 << i, i, 0
+                while up[cur] != -1:
+                    if not 0 <= up[cur] < cur:
+                        _raise(64)
+                        break
+                    cur, depth = up[cur], depth + 1
+                    bits |= 1 << cur
+            pos.append(c + depth)
+            mask.append([bits >> 32 * w & 0xffffffff for w in range(words)])
+        cu.append(cu[-1] + n)
+    for i in range(N - cu[-1]):
+        seq.append(S)
+        pos.append(i % (width * page_size))
+        kv.append(-1)
+        mask.append([0] * words)
+    ints = lambda x: torch.tensor(x, dtype=torch.int64, device=dev).to(torch.int32)
+    return StepLayout(ints(cu + [N]), ints([max(int(c), 0) for c in ctx_lens] + [0]), ints(pos), ints(seq), ints(kv),
+                      ints(tables + [[0] * width]), ints(mask).view(N, words) if words else None)
+
+
+def _bits(mask, n):
+    """[rows, n] of truth values from words of 32 bits."""
+    j = torch.arange(n, device=mask.device)
+    wide = torch.cat([mask, mask.new_zeros((mask.shape[0], max(n // 32 + 1 - mask.shape[1], 0)))], 1)
+    return (wide[:, j // 32] >> (j % 32) & 1).bool()
+
+
+def tree_attention(q, k, v, step, cache, heads, kv_heads, head_dim, scale, window=None, absolute=False):
+    """`absolute`: the weighted sum of the values' magnitudes instead (for error bounds)."""
+    H, G, D, ps = heads, kv_heads, head_dim, cache.page_size
+    out = torch.zeros((q.shape[0], H * D), dtype=torch.float64, device=q.device)
+    cu = step.cu_q.tolist()
+    for s in range(len(cu) - 1):
+        a, b, c = cu[s], cu[s + 1], max(int(step.ctx_lens[s]), 0)
+        n = b - a
+        if n <= 0:
+            continue
+        pages = _checked(cache.block_table[s, :-(-c // ps)].long(), cache.pages.shape[0], 4)
+        kv = cache.pages[pages].double().permute(1, 2, 0, 3, 4).reshape(2, G, -1, D)[:, :, :c]
+        own = torch.stack([k[a:b], v[a:b]]).double().view(2, n, G, D).transpose(1, 2)
+        kv = torch.cat([kv, own], 2)
+        pos = step.positions[a:b].long()
+        key_pos = torch.cat([torch.arange(c, device=q.device), pos])
+        sees = torch.cat([torch.ones((n, c), dtype=torch.bool, device=q.device), _bits(step.tree_mask[a:b], n)], 1)
+        if window is not None:
+            sees &= key_pos[None, :] > pos[:, None] - window
+        qs = q[a:b].double().view(n, G, H // G, D)
+        for i in range(n):
+            at = sees[i].nonzero()[:, 0]
+            if at.numel():
+                kk, vv = kv[0][:, at], kv[1][:, at]
+                p = torch.softmax(qs[i] @ kk.transpose(1, 2) * scale, -1)
+                out[a + i] = (p @ (vv.abs() if absolute else vv)).reshape(-1)
+    return out if absolute or q.dtype == torch.float64 else out.to(q.dtype)
+
+
+def accept_drafts(choices, tokens, parents, step, most):
+    from zig_ai_b200.kernels.ops import AcceptedDrafts
+    cu, S = step.cu_q.tolist(), step.cu_q.numel() - 1
+    path = torch.full((S, most), -1, dtype=torch.int32, device=choices.device)
+    chosen, counts = path.clone(), torch.zeros(S, dtype=torch.int32, device=choices.device)
+    c, t, p = choices.tolist(), tokens.tolist(), parents.tolist()
+    for s in range(S):
+        a, n = cu[s], cu[s + 1] - cu[s]
+        if n > most or any(not -1 <= p[a + i] < i for i in range(1, min(n, most))):
+            _raise(64)
+        n, cur = min(n, most), 0
+        while cur is not None and cur < n:
+            path[s, counts[s]], chosen[s, counts[s]] = a + cur, c[a + cur]
+            counts[s] += 1
+            cur = next((i for i in range(cur + 1, n) if p[a + i] == cur and t[a + i] == c[a + cur]), None)
+    return AcceptedDrafts(counts, path, chosen, step.ctx_lens + counts)
+
+
+def commit_drafts(k, v, path, counts, step, pages):
+    many = pages.dim() == 6
+    G, ps, D = pages.shape[-3:]
+    for s in range(counts.numel()):
+        for i in range(min(int(counts[s]), path.shape[1])):
+            row, slot = int(path[s, i]), int(step.kv_slots[int(step.cu_q[s]) + i])
+            if slot < 0:
+                continue
+            for which, x in ((0, k), (1, v)):
+                if many:
+                    pages[:, slot // ps, which, :, slot % ps] = x[:, row].reshape(-1, G, D)
+                else:
+                    pages[slot // ps, which, :, slot % ps] = x[row].view(G, D)

@@ -1,0 +1,546 @@
+"""The kernels of a step that checks drafted tokens (step tables, tree attention, log probabilities, the accepted path, the accepted
+rows' keys and values) against plain versions in 64 bits (tests/ref_ops.py)."""
+import random
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+import ref_ops
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def ops():
+    from zig_ai_b200.kernels import ops as o
+    return o
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def make_parents(g, n, shape="mixed"):
+    if shape == "chain":
+        return [i - 1 for i in range(n)]
+    if n == 0:
+        return []
+    if shape == "star":
+        return [-1] + [0] * (n - 1)
+    if shape == "forest":
+        return [-1 if i == 0 or g.random() < 0.3 else g.randrange(i) for i in range(n)]
+    return [-1] + [max(i - 1 - g.randrange(4), 0) for i in range(1, n)]
+
+
+def make_masks(parents_by_span, words):
+    rows, depths = [], []
+    for parents in parents_by_span:
+        bits, depth = [], []
+        for i, p in enumerate(parents):
+            bits.append((bits[p] if p >= 0 else 0) | 1 << i)
+            depth.append(depth[p] + 1 if p >= 0 else 0)
+        rows += [[b >> 32 * w & 0xffffffff for w in range(words)] for b in bits]
+        depths.append(depth)
+    return torch.tensor(rows, dtype=torch.int64).to(torch.int32).view(-1, words).cuda(), depths
+
+
+def make_tree_step(q_lens, ctx, H, G, D, ps, dtype, seed, shape="mixed", extra_words=0, poison=float("nan"), packed=True):
+    """A step of trees behind random block tables; everything of the pages that no row may look at is `poison`."""
+    g, t = random.Random(seed), torch.Generator(device="cuda").manual_seed(seed)
+    S, N = len(q_lens), sum(q_lens)
+    parents = [make_parents(g, n, shape) for n in q_lens]
+    words = max(-(-max(q_lens + [1]) // 32), 1) + extra_words
+    mask, depths = make_masks(parents, words)
+    width = max(max(-(-(c + n) // ps) for c, n in zip(ctx, q_lens)), 1)
+    held = [-(-c // ps) for c in ctx]
+    ids = list(range(1, sum(held) + 3))
+    g.shuffle(ids)
+    table, pages = [], torch.full((sum(held) + 3, 2, G, ps, D), poison, dtype=dtype, device="cuda")
+    for c, n in zip(ctx, held):
+        row = [ids.pop() for _ in range(n)]
+        for j, p in enumerate(row):
+            m = min(ps, c - j * ps)
+            pages[p, :, :, :m] = torch.randn((2, G, m, D), generator=t, device="cuda").to(dtype)
+        table.append(row + [0] * (width - n))
+    q = (2 * torch.randn((N, H * D), generator=t, device="cuda")).to(dtype)
+    qkv = torch.randn((N, (H + 2 * G) * D), generator=t, device="cuda").to(dtype)
+    k, v = qkv[:, H * D:(H + G) * D], qkv[:, (H + G) * D:]
+    if packed:
+        k, v = k.contiguous(), v.contiguous()
+    cu = [0]
+    for n in q_lens:
+        cu.append(cu[-1] + n)
+    step = SimpleNamespace(cu_q=ints(cu), ctx_lens=ints(ctx), positions=ints([c + d for c, ds in zip(ctx, depths) for d in ds]), tree_mask=mask,
+                           n_seqs=S, n_tokens=N, max_q_len=max(q_lens), q_lens=q_lens)
+    return q, k, v, step, SimpleNamespace(pages=pages, block_table=ints(table), page_size=ps), parents
+
+
+def close(got, q, k, v, step, cache, H, G, D, scale, window):
+    """Against 64 bits.  With u the half step of 32 bits (2^-24) a score is off by at most d = (D + 4) u sum|q k| scale (products and sums in any
+    order) and a few u of itself in the exponential's argument; a weight by a factor e^(2 d) and 8 u, the sums by the number of
+    keys times u: |o - o64| <= sum p|v| (2 d + (keys + 16) u), and in bfloat16 half a step of 2^-8 for the weights (times sum
+    p|v|) and one for the result."""
+    want = ref_ops.tree_attention(q, k, v, step, cache, H, G, D, scale, window)
+    exact = ref_ops.tree_attention(q.double(), k, v, step, cache, H, G, D, scale, window)
+    size = ref_ops.tree_attention(q.double(), k, v, step, cache, H, G, D, scale, window, absolute=True)
+    assert got.dtype == q.dtype and got.shape == want.shape
+    u, keys = 2.0 ** -24, max(int(step.ctx_lens.max()), 0) + step.max_q_len
+    kmax = max(float(cache.pages[:, 0].double().nan_to_num().abs().max()), float(k.double().nan_to_num().abs().max()))
+    score = float(q.double().abs().view(-1, D).sum(1).max()) * kmax * scale
+    bound = size * (2 * (D + 8) * u * score + (keys + 16) * u)
+    if q.dtype == BF16:
+        bound = bound + 2.0 ** -8 * size + 2.0 ** -8 * exact.abs()
+    over = (got.double() - exact).abs() - bound
+    assert torch.isfinite(got).all()
+    assert float(over.max()) <= 0, (float(over.max()), float((got.double() - exact).abs().max()))
+
+
+TREES = [
+    # q_lens, ctx, H, G, D, page, window
+    ([1], [0], 2, 2, 64, 16, None),                            # one row that sees itself alone
+    ([1], [1], 4, 1, 64, 16, None),
+    ([5], [63], 8, 2, 64, 64, None),
+    ([12], [1000], 16, 8, 64, 64, None),
+    ([3, 1, 9, 24, 2], [64, 0, 129, 500, 17], 8, 2, 64, 16, None),
+    ([33, 64, 65], [100, 31, 640], 8, 2, 64, 32, None),        # masks of several words, tiles of pairs that end inside a row's heads
+    ([40], [300], 3, 1, 64, 8, None),                          # three heads share a key/value head
+    ([70, 3], [257, 2000], 16, 2, 128, 64, None),
+    ([7, 11], [333, 90], 4, 4, 128, 16, 50),                   # windows: inside the cache, inside the tree
+    ([20, 33], [400, 3], 8, 4, 64, 16, 7),
+    ([6, 2], [64, 65], 4, 2, 96, 16, None),
+    ([9, 4], [130, 5], 6, 2, 32, 4, 40),
+    ([5, 8], [77, 12], 6, 3, 80, 16, None),                    # the general kernel's head sizes
+    ([4, 3], [40, 19], 2, 1, 13, 5, None),
+    ([3], [21], 2, 2, 320, 8, 9),
+    ([130], [40], 2, 1, 64, 16, None),                         # a large tree
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("q_lens,ctx,H,G,D,ps,window", TREES)
+def test_tree_attention(dtype, q_lens, ctx, H, G, D, ps, window):
+    for shape in ("mixed", "forest"):
+        q, k, v, step, cache, _ = make_tree_step(list(q_lens), list(ctx), H, G, D, ps, dtype, 7, shape, packed=shape == "mixed")
+        got = ops().tree_attention(q, k, v, step, cache, H, G, D, D ** -0.5, window)
+        close(got, q, k, v, step, cache, H, G, D, D ** -0.5, window)
+    assert ops().read_status() == 0
+
+
+@pytest.mark.parametrize("dtype,impl", [(F32, None), (BF16, "general"), (BF16, "mma")])
+@pytest.mark.parametrize("splits", [1, 2, 4, 8, 16])
+@pytest.mark.parametrize("D,group,n", [(64, 2, 5), (64, 4, 8), (64, 4, 14), (128, 4, 30), (128, 8, 2)])
+def test_tree_attention_by_every_split(dtype, impl, splits, D, group, n):
+    """Every number of blocks that share a tile's keys, more than there are tiles among them."""
+    q, k, v, step, cache, _ = make_tree_step([n, 1, n], [700, 3, 129], 2 * group, 2, D, 16, dtype, 11, extra_words=2)
+    got = ops().tree_attention(q, k, v, step, cache, 2 * group, 2, D, D ** -0.5, impl=impl, splits=splits)
+    close(got, q, k, v, step, cache, 2 * group, 2, D, D ** -0.5, None)
+
+
+@pytest.mark.parametrize("dtype,impl", [(F32, None), (BF16, "general"), (BF16, "mma")])
+@pytest.mark.parametrize("splits", [1, 4])
+def test_rows_that_see_nothing_and_empty_spans(dtype, impl, splits):
+    """A mask without bits over an empty cache gives zeros; spans without rows take no part."""
+    q, k, v, step, cache, _ = make_tree_step([4, 6, 3], [0, 50, 0], 4, 2, 64, 16, dtype, 3)
+    step.tree_mask[1] = 0
+    step.tree_mask[10:13] = 0
+    step.cu_q = ints([0, 4, 4, 10, 13, 13])
+    step.ctx_lens, step.n_seqs = ints([0, 900, 50, 0, 7]), 5
+    cache.block_table = cache.block_table[[0, 1, 1, 2, 1]].contiguous()
+    got = ops().tree_attention(q, k, v, step, cache, 4, 2, 64, 0.125, impl=impl, splits=splits)
+    close(got, q, k, v, step, cache, 4, 2, 64, 0.125, None)
+    assert not got[[1, 10, 11, 12]].any()
+
+
+@pytest.mark.parametrize("dtype,impl", [(F32, None), (BF16, "general"), (BF16, "mma")])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_what_is_not_finite_reaches_the_rows_that_see_it_alone(dtype, impl, bad):
+    H, G, D = 4, 2, 64
+    q, k, v, step, cache, parents = make_tree_step([9, 70], [100, 40], H, G, D, 16, dtype, 5)
+    want = ops().tree_attention(q, k, v, step, cache, H, G, D, 0.125, impl=impl, splits=2)
+    k, v = k.clone(), v.clone()
+    k[4] = bad                                              # row 4 of the first tree, row 60 of the second
+    v[9 + 60, :D] = bad
+    got = ops().tree_attention(q, k, v, step, cache, H, G, D, 0.125, impl=impl, splits=2)
+    sees = ref_ops._bits(step.tree_mask, 70)
+    hit = torch.zeros((79, H, D), dtype=torch.bool, device="cuda")
+    hit[:9][sees[:9, 4]] = True
+    hit[9:, :H // G][sees[9:, 60]] = True                     # (the first key/value head's query heads)
+    hit = hit.view(79, -1)
+    assert torch.equal(got[~hit], want[~hit])
+    assert not torch.isfinite(got[hit]).any()
+    # a window's edge inside a tile of cached keys
+    q, k, v, step, cache, _ = make_tree_step([6], [90], H, G, D, 16, dtype, 6, "chain")
+    clean = ops().tree_attention(q, k, v, step, cache, H, G, D, 0.125, 20, impl=impl, splits=1)
+    page, off = int(cache.block_table[0, 72 // 16]), 72 % 16
+    cache.pages[page, 1, :, off] = bad                       # position 72: rows at 90 and 91 see it (72 > 91 - 20), those behind do not
+    got = ops().tree_attention(q, k, v, step, cache, H, G, D, 0.125, 20, impl=impl, splits=1)
+    assert torch.equal(got[2:], clean[2:]) and not torch.isfinite(got[:2]).any()
+
+
+def test_tree_attention_large_offsets():
+    """A pool whose later pages lie beyond 2^31 elements."""
+    H, G, D, ps = 4, 2, 64, 64
+    per_page = 2 * G * ps * D
+    n_pages = (1 << 31) // per_page + 40
+    pages = torch.empty((n_pages, 2, G, ps, D), dtype=BF16, device="cuda")
+    q, k, v, step, cache, _ = make_tree_step([5, 3], [200, 130], H, G, D, ps, BF16, 9)
+    used = cache.pages.shape[0]
+    pages[-used:] = cache.pages
+    pages[0] = float("nan")
+    want = ops().tree_attention(q, k, v, step, cache, H, G, D, 0.125)
+    far = SimpleNamespace(pages=pages, page_size=ps, block_table=torch.where(cache.block_table > 0, cache.block_table + n_pages - used, 0).int())
+    for impl in ("mma", "general"):
+        near = ops().tree_attention(q, k, v, step, cache, H, G, D, 0.125, impl=impl)
+        assert torch.equal(ops().tree_attention(q, k, v, step, far, H, G, D, 0.125, impl=impl), near)
+    assert want.isfinite().all()
+
+
+def test_bad_pages_raise_the_status_word():
+    q, k, v, step, cache, _ = make_tree_step([5, 3], [200, 130], 4, 2, 64, 16, BF16, 9, poison=0.0)
+    good = ops().tree_attention(q, k, v, step, cache, 4, 2, 64, 0.125)
+    assert ops().read_status() == 0
+    bt = cache.block_table.clone()
+    bt[0, 3] = cache.pages.shape[0]
+    for impl in ("mma", "general"):
+        got = ops().tree_attention(q, k, v, step, SimpleNamespace(pages=cache.pages, block_table=bt, page_size=16), 4, 2, 64, 0.125, impl=impl)
+        assert ops().read_status() == 4
+        if impl == "mma":
+            assert torch.equal(got[5:], good[5:])
+    narrow = SimpleNamespace(pages=cache.pages, block_table=cache.block_table[:, :5].contiguous(), page_size=16)
+    ops().tree_attention(q, k, v, step, narrow, 4, 2, 64, 0.125)
+    assert ops().read_status() == 16
+    step.cu_q = ints([0, 5, 99])
+    step.n_seqs = 2
+    ops().tree_attention(q, k, v, step, cache, 4, 2, 64, 0.125)
+    assert ops().read_status() == 32
+
+
+def test_unaligned_rows_take_the_general_kernel():
+    q, k, v, step, cache, _ = make_tree_step([5, 3], [20, 130], 4, 2, 64, 16, BF16, 9)
+    wide = torch.zeros((8, 2 * 64 + 3), dtype=BF16, device="cuda")
+    wide[:, 1:129] = k
+    got = ops().tree_attention(q, wide[:, 1:129], v, step, cache, 4, 2, 64, 0.125)
+    close(got, q, k, v, step, cache, 4, 2, 64, 0.125, None)
+    with pytest.raises(ops().KernelError, match="16-byte"):
+        ops().tree_attention(q, wide[:, 1:129], v, step, cache, 4, 2, 64, 0.125, impl="mma")
+
+
+def test_tree_attention_refuses():
+    q, k, v, step, cache, _ = make_tree_step([5, 3], [20, 130], 4, 2, 64, 16, BF16, 9)
+    o = ops()
+
+    def call(**kw):
+        a = dict(q=q, k=k, v=v, step=step, cache=cache, heads=4, kv_heads=2, head_dim=64, scale=0.125, window=None)
+        a.update(kw)
+        with pytest.raises(o.KernelError):
+            o.tree_attention(**a)
+
+    def but(ns, **kw):
+        return SimpleNamespace(**{**vars(ns), **kw})
+
+    call(kv_heads=3)
+    call(q=q.float())
+    call(k=k[:, :64])
+    call(v=v[:4])
+    call(scale=0.0)
+    call(scale=float("nan"))
+    call(window=0)
+    call(step=but(step, tree_mask=None))
+    call(step=but(step, tree_mask=step.tree_mask[:3]))
+    call(step=but(step, tree_mask=step.tree_mask.long()))
+    call(step=but(step, ctx_lens=step.ctx_lens[:1]))
+    call(step=but(step, n_tokens=9))
+    call(step=but(step, positions=step.positions[:5]))
+    call(cache=but(cache, pages=cache.pages.float()))
+    call(cache=but(cache, page_size=8))
+    call(cache=but(cache, block_table=cache.block_table[:1]))
+    call(q=q.cpu())
+    call(splits=3 * 16)
+    empty = but(step, n_tokens=0, tree_mask=step.tree_mask[:0], positions=step.positions[:0], cu_q=ints([0, 0, 0]))
+    assert o.tree_attention(q[:0], k[:0], v[:0], empty, cache, 4, 2, 64, 0.125).shape == (0, 256)
+
+
+# ------------------------------------------------------------------------------------------------ log probabilities
+def check_logprobs(x, t, top, **kw):
+    got, want = ops().token_logprobs(x, t, top, **kw), ref_ops.token_logprobs(x, t, top)
+    assert torch.equal(got.ranks, want.ranks) and torch.equal(got.top_ids, want.top_ids)
+    # 32 bits: differences from the maximum are off by half a step of themselves, at most 2^-24 of the row's spread; ln z by the relative error of
+    # z (a few steps of the exponential, V / 512 terms a thread one after the other); the entropy by that of u as well
+    spread = (x.double().amax(1) - torch.where(x.double() == float("-inf"), x.double().amax(1, keepdim=True), x.double()).amin(1)).clamp(1.0, 200.0)
+    tol = 2.0 ** -24 * (spread * 4 + 8 + x.shape[1] / 128)
+    for a, b in ((got.logprobs, want.logprobs), (got.entropy, want.entropy)):
+        far = (a.double() - b).abs()
+        assert bool(((far <= tol + 2.0 ** -23 * b.abs()) | (a.double() == b)).all()), float(far.max())
+    far = (got.top_logprobs.double() - want.top_logprobs).abs()
+    assert bool(((far <= tol[:, None] + 2.0 ** -23 * want.top_logprobs.abs()) | (got.top_logprobs.double() == want.top_logprobs)).all())
+    return got
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("R,V,top", [(1, 1, 0), (1, 1, 1), (3, 2, 2), (2, 31, 5), (5, 32, 32), (1, 777, 20), (4, 8191, 1), (3, 8192, 32), (2, 8193, 5),
+                                     (7, 65536, 20), (33, 50001, 3), (160, 20003, 8), (400, 3001, 0), (1, 200001, 32)])
+def test_token_logprobs(dtype, R, V, top):
+    g = torch.Generator(device="cuda").manual_seed(R * 1000 + V)
+    x = (3 * torch.randn((R, V), generator=g, device="cuda")).to(dtype)
+    t = torch.randint(0, V, (R,), generator=g, device="cuda", dtype=torch.int32)
+    t[0] = V - 1
+    check_logprobs(x, t, top)
+
+
+@pytest.mark.parametrize("blocks", [1, 2, 4, 8, 16])
+@pytest.mark.parametrize("V", [5, 70000, 33333])
+def test_token_logprobs_by_every_split(blocks, V):
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = 2 * torch.randn((3, V), generator=g, device="cuda")
+    check_logprobs(x, ints([0, V - 1, V // 2]), 5, blocks=blocks)
+    assert torch.equal(ops().token_logprobs(x, ints([0, V - 1, V // 2]), 5, blocks=blocks).logprobs,
+                       ops().token_logprobs(x, ints([0, V - 1, V // 2]), 5, blocks=blocks).logprobs)
+
+
+@pytest.mark.parametrize("blocks", [0, 1, 4])
+def test_token_logprobs_of_unusual_rows(blocks):
+    """Ties, rows that ascend or descend, masked tokens (-inf and the type's lowest value), a single token left."""
+    V = 40000
+    j = torch.arange(V, device="cuda").float()
+    low = torch.finfo(F32).min
+    rows = [torch.zeros(V, device="cuda"), j / V, -j / V, (j % 7).clone(), torch.full((V,), low, device="cuda")]
+    masked = torch.full((V,), float("-inf"), device="cuda")
+    masked[[39, 20000, V - 1]] = torch.tensor([1.0, 1.0, -2.0], device="cuda")
+    lowest = torch.full((V,), low, device="cuda")
+    lowest[[5, 30000]] = torch.tensor([2.0, 3.0], device="cuda")
+    only = torch.full((V,), float("-inf"), device="cuda")
+    only[17] = -4.0
+    signed = torch.where(j % 2 == 0, -0.0, 0.0)
+    peak = torch.randn(V, device="cuda")
+    peak[12345] = 120.0
+    x = torch.stack(rows + [masked, lowest, only, signed, peak])
+    for t in ([0, V - 1, V - 1, 6, 100, 20000, 5, 17, 1, 12345], [V - 1, 0, 0, 13, 0, 39, 30000, 17, 0, 1]):
+        check_logprobs(x, ints(t), 20, blocks=blocks)
+    got = ops().token_logprobs(x, ints([-1] * 10), 3, blocks=blocks)
+    assert got.logprobs.tolist() == [0.0] * 10 and got.ranks.tolist() == [-1] * 10
+    masked_token = ops().token_logprobs(x[5:6], ints([3]), 0, blocks=blocks)
+    assert masked_token.logprobs.tolist() == [float("-inf")] and masked_token.ranks.tolist() == [3 + 3]       # three tokens that can come, three before it that cannot
+    assert ops().read_status() == 0
+
+
+def test_token_logprobs_of_rows_without_a_distribution():
+    V = 9000
+    x = torch.randn((4, V), device="cuda")
+    x[0] = float("-inf")
+    x[1, 4000] = float("inf")
+    x[2, 17] = float("nan")
+    got = ops().token_logprobs(x, ints([1, 2, 3, 4]), 4)
+    assert torch.isnan(got.logprobs[[0, 1, 2]]).all() and torch.isnan(got.entropy[[0, 1, 2]]).all()
+    assert bool(((got.top_ids >= 0) & (got.top_ids < V)).all())
+    assert torch.isfinite(got.logprobs[3])
+
+
+def test_token_logprobs_of_strided_rows_and_tokens_outside():
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for dtype in (F32, BF16):
+        wide = torch.randn((6, 5003), generator=g, device="cuda").to(dtype)
+        check_logprobs(wide[:, 2:4500], ints([0, 1, 2, 3, 4, 4497]), 6)
+        check_logprobs(wide[::2, 1:], ints([5, 6, 7]), 6)
+    x = torch.randn((3, 100), generator=g, device="cuda")
+    got = ops().token_logprobs(x, ints([100, 4, -2]), 2)
+    assert ops().read_status() == 2
+    assert got.ranks.tolist()[::2] == [-1, -1] and got.logprobs.tolist()[::2] == [0.0, 0.0]
+    assert got.logprobs[1] == ops().token_logprobs(x, ints([4, 4, 4]), 0).logprobs[1]
+
+
+def test_token_logprobs_refuses():
+    x, t = torch.randn((3, 50), device="cuda"), ints([0, 1, 2])
+    o = ops()
+    for bad in (lambda: o.token_logprobs(x, t, 33), lambda: o.token_logprobs(x[:, :4], t, 5), lambda: o.token_logprobs(x, t, -1),
+                lambda: o.token_logprobs(x, t.long(), 1), lambda: o.token_logprobs(x, t[:2], 1), lambda: o.token_logprobs(x.half(), t, 1),
+                lambda: o.token_logprobs(x.t(), t, 1), lambda: o.token_logprobs(x.cpu(), t, 1), lambda: o.token_logprobs(x, t.cpu(), 1),
+                lambda: o.token_logprobs(x, t, 1, blocks=3), lambda: o.token_logprobs(x, t, 1, blocks=32)):
+        with pytest.raises(o.KernelError):
+            bad()
+    assert o.token_logprobs(x[:0], t[:0], 4).top_ids.shape == (0, 4)
+
+
+# ------------------------------------------------------------------------------------------------ the step's tables
+def same_layout(got, want):
+    for name, a, b in zip(got._fields, got, want):
+        assert (a is None) == (b is None), name
+        if a is not None:
+            assert a.dtype == torch.int32 and torch.equal(a.cpu(), b.cpu()), name
+
+
+@pytest.mark.parametrize("q_lens,spare,tree", [([1], 0, True), ([1], 0, False), ([5, 0, 3, 1, 0], 7, True), ([0, 0], 4, True), ([3, 300, 40], 0, False),
+                                               ([64, 33, 1, 32, 100], 31, True), ([1] * 300, 3, False), ([2] * 70, 0, True), ([1000], 24, True),
+                                               ([], 3, False)])
+@pytest.mark.parametrize("shape", ["mixed", "chain", "forest"])
+def test_step_layout(q_lens, spare, tree, shape):
+    g = random.Random(len(q_lens) + spare)
+    S, N, ps = len(q_lens), sum(q_lens) + spare, 16
+    ctx = [g.choice([0, 1, 15, 16, 17, 400]) for _ in q_lens]
+    width = max([-(-(c + n) // ps) for c, n in zip(ctx, q_lens)] + [1]) + 1
+    slots = g.sample(range(S + 5), S)
+    rows = torch.tensor([[g.randrange(1, 9999) for _ in range(width + 2)] for _ in range(S + 5)], dtype=torch.int32)
+    parents = torch.tensor([p for n in q_lens for p in make_parents(g, n, shape)] + [-1] * spare, dtype=torch.int32) if tree else None
+    most = max(q_lens + [1])
+    cpu = [torch.tensor(x, dtype=torch.int32) for x in (q_lens, ctx, slots)] + [rows]
+    got = ops().step_layout(*[x.cuda() for x in cpu], ps, N, width, parents.cuda() if tree else None, most)
+    want = ref_ops.step_layout(*cpu, ps, N, width, parents, most)
+    same_layout(got, want)
+    assert ops().read_status() == 0
+
+
+def test_step_layout_raises_the_status_word():
+    rows = torch.arange(1, 41, dtype=torch.int32).view(4, 10)
+
+    def both(code, q, c, s, n, width=10, parents=None, most=0, rows=rows):
+        cpu = [torch.tensor(x, dtype=torch.int32) for x in (q, c, s)] + [rows]
+        up = None if parents is None else torch.tensor(parents, dtype=torch.int32)
+        ref_ops.read_status()
+        same_layout(ops().step_layout(*[x.cuda() for x in cpu], 4, n, width, None if up is None else up.cuda(), most),
+                    ref_ops.step_layout(*cpu, 4, n, width, up, most))
+        assert ops().read_status() == code and ref_ops.read_status() == code
+
+    both(0, [3, 2], [1, 2], [0, 3], 6)
+    both(32, [3, 9, 1], [1, 2, 0], [0, 3, 1], 6)              # more rows than there is room for
+    both(32, [3, -2, 1], [1, 2, 0], [0, 3, 1], 6)
+    both(8, [3, 2], [1, 2], [0, 4], 6)                        # a slot outside the slots
+    both(8, [3, 2], [1, 2], [-1, 1], 6)
+    both(16, [3, 2], [1, 39], [0, 1], 6)                      # a position outside the block table
+    both(16, [3, 2], [1, 7], [0, 1], 6, width=2)
+    both(16, [3, 2], [-1, 7], [0, 1], 6)
+    both(64, [3, 2], [1, 2], [0, 1], 5, parents=[-1, 1, 0, -1, 0], most=4)         # hangs on itself
+    both(64, [3, 2], [1, 2], [0, 1], 5, parents=[-1, 0, -5, -1, 0], most=4)
+    both(64, [4, 2], [1, 2], [0, 1], 6, parents=[-1, 0, 1, 2, -1, 0], most=3)      # a tree of more rows than it may have
+    both(4, [3, 2], [1, 2], [0, 1], 5, rows=-rows)
+
+
+def test_step_layout_refuses():
+    o, one, rows = ops(), ints([1]), ints([[1, 2]])
+    ok = dict(q_lens=one, ctx_lens=one, slots=ints([0]), page_rows=rows, page_size=4, n_rows=1, width=2)
+    o.step_layout(**ok)
+    for kw in (dict(q_lens=one.cpu()), dict(q_lens=one.long()), dict(ctx_lens=ints([1, 2])), dict(slots=ints([[0]])), dict(page_rows=ints([1, 2])),
+               dict(page_size=0), dict(width=0), dict(n_rows=-1), dict(parents=ints([-1]), tree_rows=0), dict(parents=ints([-1]), tree_rows=1025),
+               dict(parents=ints([-1, 0]), tree_rows=4), dict(n_rows=1 << 22), dict(width=1 << 30, page_size=1 << 10)):
+        with pytest.raises((o.KernelError, RuntimeError)):
+            o.step_layout(**{**ok, **kw})
+    assert o.read_status() == 0
+
+
+# ------------------------------------------------------------------------------------------------ the accepted path
+@pytest.mark.parametrize("q_lens,vocab", [([1], 5), ([2, 1, 6], 3), ([12, 0, 7, 33], 4), ([64, 40, 1, 200], 6), ([5] * 100, 2), ([1024], 2)])
+@pytest.mark.parametrize("shape", ["mixed", "chain", "star", "forest"])
+def test_accept_drafts(q_lens, vocab, shape):
+    g = random.Random(sum(q_lens) + vocab)
+    parents = [p for n in q_lens for p in make_parents(g, n, shape)]
+    N, cu = len(parents), [0]
+    for n in q_lens:
+        cu.append(cu[-1] + n)
+    tokens, choices = ([g.randrange(vocab) for _ in range(N)] for _ in range(2))
+    step = SimpleNamespace(cu_q=ints(cu), ctx_lens=ints([g.randrange(100) for _ in q_lens]))
+    args = (ints(choices), ints(tokens), ints(parents), step, max(q_lens))
+    got, want = ops().accept_drafts(*args), ref_ops.accept_drafts(*args)
+    for name, a, b in zip(got._fields, got, want):
+        assert a.dtype == torch.int32 and torch.equal(a, b), name
+    assert ops().read_status() == 0
+    assert all(int(c) >= 1 for c, n in zip(got.counts, q_lens) if n)
+
+
+def test_accept_drafts_raises_and_refuses():
+    o = ops()
+    step = SimpleNamespace(cu_q=ints([0, 3, 5]), ctx_lens=ints([4, 9]))
+    a = [ints([7, 7, 7, 7, 7]), ints([7, 7, 7, 7, 7]), ints([-1, 0, 2, -1, 0])]
+    got = o.accept_drafts(*a, step, 3)
+    assert o.read_status() == 64 and got.counts.tolist() == [2, 2]
+    got = o.accept_drafts(a[0], a[1], ints([-1, 0, 1, -1, 0]), step, 2)
+    assert o.read_status() == 64 and got.counts.tolist() == [2, 2] and got.path.shape == (2, 2)
+    bad = SimpleNamespace(cu_q=ints([0, 3, 9]), ctx_lens=step.ctx_lens)
+    got = o.accept_drafts(a[0], a[1], ints([-1, 0, 1, -1, 0]), bad, 6)
+    assert o.read_status() == 32 and got.counts.tolist() == [3, 0]
+    for args in ((a[0][:4], a[1], a[2], step, 3), (a[0], a[1].long(), a[2], step, 3), (*a, step, 0), (*a, step, 2000),
+                 (*a, SimpleNamespace(cu_q=step.cu_q, ctx_lens=ints([1])), 3), (a[0].cpu(), a[1], a[2], step, 3)):
+        with pytest.raises(o.KernelError):
+            o.accept_drafts(*args)
+
+
+# ------------------------------------------------------------------------------------------------ accepted rows into the pages
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("planes,G,D,ps,strided", [(0, 2, 64, 16, False), (0, 2, 64, 16, True), (3, 8, 64, 64, False), (2, 1, 13, 5, False),
+                                                   (1, 3, 20, 4, True), (0, 4, 128, 32, True), (2, 2, 320, 8, False)])
+def test_commit_drafts(dtype, planes, G, D, ps, strided):
+    g, t = random.Random(D), torch.Generator(device="cuda").manual_seed(D)
+    q_lens, ctx = [5, 1, 9, 0, 30], [0, 15, 16, 3, 77]
+    S, N, cu = len(q_lens), sum(q_lens), [0]
+    for n in q_lens:
+        cu.append(cu[-1] + n)
+    ids = list(range(1, 400))
+    g.shuffle(ids)
+    table = [[ids.pop() for _ in range(-(-(c + n) // ps) + 1)] for c, n in zip(ctx, q_lens)]
+    slots = [table[s][(ctx[s] + i) // ps] * ps + (ctx[s] + i) % ps for s in range(S) for i in range(q_lens[s])]
+    slots[3] = -1                                              # a row without a place
+    counts = [n if s == 0 else (n + 1) // 2 for s, n in enumerate(q_lens)]
+    path = [sorted(g.sample(range(cu[s], cu[s + 1]), c)) + [-1] * (max(q_lens) - c) for s, c in enumerate(counts)]
+    lead = (planes,) if planes else ()
+    pages = torch.randn(lead + (400, 2, G, ps, D), generator=t, device="cuda").to(dtype)
+    rows = torch.randn(lead + (N, 3 * G * D + 1), generator=t, device="cuda").to(dtype)
+    k, v = rows[..., :G * D], rows[..., G * D:2 * G * D]
+    if not strided:
+        k, v = k.contiguous(), v.contiguous()
+    step = SimpleNamespace(cu_q=ints(cu), kv_slots=ints(slots))
+    want = pages.clone()
+    ref_ops.commit_drafts(k, v, ints(path), ints(counts), step, want)
+    ops().commit_drafts(k, v, ints(path), ints(counts), step, pages)
+    assert torch.equal(pages, want)
+    assert ops().read_status() == 0
+
+
+def test_commit_drafts_raises_and_refuses():
+    o = ops()
+    pages, k = torch.zeros((6, 2, 1, 4, 8), dtype=BF16, device="cuda"), torch.ones((3, 8), dtype=BF16, device="cuda")
+    step = SimpleNamespace(cu_q=ints([0, 3]), kv_slots=ints([4, 5, 24]))
+    o.commit_drafts(k, k, ints([[0, 1, 2]]), ints([2]), step, pages)
+    assert o.read_status() == 0 and int((pages != 0).sum()) == 32
+    for path, counts, slots, code in (([[0, 1, 2]], [3], [4, 5, 24], 4), ([[0, 3, 1]], [2], [4, 5, 6], 32), ([[0, -1, 1]], [2], [4, 5, 6], 32),
+                                      ([[0, 1, 2]], [4], [4, 5, 6], 32)):
+        o.commit_drafts(k, k, ints(path), ints(counts), SimpleNamespace(cu_q=step.cu_q, kv_slots=ints(slots)), pages.clone())
+        assert o.read_status() == code
+    a = dict(k=k, v=k, path=ints([[0, 1, 2]]), counts=ints([2]), step=step, pages=pages)
+    for kw in (dict(k=k.float()), dict(v=k[:2]), dict(pages=pages[0]), dict(pages=pages.float()), dict(path=ints([0, 1])), dict(counts=ints([1, 1])),
+               dict(pages=torch.zeros((6, 1, 2, 4, 8), dtype=BF16, device="cuda")), dict(path=ints([[0]]).long()), dict(k=k.cpu())):
+        with pytest.raises(o.KernelError):
+            o.commit_drafts(**{**a, **kw})
+    assert o.read_status() == 0
+
+
+# ------------------------------------------------------------------------------------------------ streams and graphs
+def test_operators_on_another_stream_and_in_graphs():
+    """Two captured graphs of the same operators, replayed in turn and on two streams at once, keep nothing of one another."""
+    o = ops()
+    sets = []
+    for seed, ctx in ((1, [300, 90]), (2, [40, 700])):
+        q, k, v, step, cache, parents = make_tree_step([6, 9], ctx, 8, 2, 64, 16, BF16, seed)
+        x, t = torch.randn((15, 9001), device="cuda"), ints([seed] * 15)
+        up, tok = ints([p for ps in parents for p in ps]), ints([i % 3 for i in range(15)])
+
+        def call(q=q, k=k, v=v, step=step, cache=cache, x=x, t=t, up=up, tok=tok):
+            return [o.tree_attention(q, k, v, step, cache, 8, 2, 64, 0.125), *o.token_logprobs(x, t, 5), *o.accept_drafts(o.argmax(x) % 3, tok, up, step, 9)]
+        call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        sets.append((call, graph, out))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(20):
+        for st, (_, graph, _) in zip(streams, sets):
+            with torch.cuda.stream(st):
+                graph.replay()
+    torch.cuda.synchronize()
+    for call, _, out in sets:
+        with torch.cuda.stream(streams[0]):
+            want = call()
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
+    assert o.read_status() == 0

@@ -1,0 +1,385 @@
+// Log probabilities of given tokens, with a row's entropy, the tokens' ranks and the best alternatives, in one walk over the logits.
+//
+// For a row x[0..V) and a token t, with m = max x, z = sum exp(x - m), u = sum (x - m) exp(x - m):
+//     logprob(j) = x[j] - m - ln z          entropy = ln z - u / z
+//     rank(t)    = how many j stand before t in the order by value, equal values by the lower index
+//     top        = the first `top` of that order
+// A thread keeps m, z, u of what it has seen (rescaled when its maximum grows) and the count for the rank; they are joined at the end.
+//
+// The best tokens.  An entry's key is its value's bits in an order that compares as a whole number, and behind them the complement
+// of its index: keys are all different, and the order of keys is the order wanted.  The first round of the walk (a piece of the row) is split into 32
+// groups by lane; the top-th largest of the groups' largest keys bounds the row's top-th key from below (`top` <= 32), so from then on only keys at or
+// above it are noted in shared memory: some thirty of the first 8192 entries and fewer of each later round, unless the row ascends.  At the end
+// a noted key's rank is the number of noted keys above it.  A row that notes more than there is room for is walked again in steps that
+// cut the list down and raise the bound as they go.
+//
+// A row is split over a cluster of up to 16 blocks when there are few rows; the first block joins the parts through distributed shared memory.
+#include <cooperative_groups.h>
+#include "common.cuh"
+namespace cg = cooperative_groups;
+
+#define LP_THREADS 512
+#define LP_WARPS (LP_THREADS / 32)
+#define LP_ROUND 16                 // entries of a row a thread looks at in one round
+#define LP_ROOM 1024                // noted keys a block has room for
+#define LP_PART 64                  // noted keys a block of a cluster may hand on (16 blocks: LP_ROOM)
+typedef unsigned long long u64;
+
+__device__ __forceinline__ u64 key_of(float x, int j) {
+    const int b = __float_as_int(x + 0.f);                     // (-0 counts as 0; what is not a number comes last)
+    const unsigned order = x != x ? 0u : (unsigned)(b ^ (b >> 31 & 0x7fffffff)) ^ 0x80000000u;
+    return ((u64)order << 32) | (unsigned)~j;
+}
+__device__ __forceinline__ float value_of(u64 key) {
+    const int o = (int)((unsigned)(key >> 32) ^ 0x80000000u);
+    return __int_as_float(o ^ (o >> 31 & 0x7fffffff));
+}
+// e^x, 2 ulp of 2^(x log2 e) beside the rounding of the product (x <= 0 here; large -x, where that shows, weigh nothing)
+__device__ __forceinline__ float exp_of(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+    return y;
+}
+
+struct Sums { float m, z, u; };
+// a's sums with b's: each relative to its own maximum
+__device__ __forceinline__ Sums joined(const Sums& a, const Sums& b) {
+    const float m = fmaxf(a.m, b.m);
+    Sums r = {m, 0.f, 0.f};
+    if (a.m != -INFINITY) {
+        const float d = fmaxf(a.m - m, -150.f), f = exp_of(d);     // (0 beyond that, which a difference near the type's end must not turn into NaN)
+        r.z += f * a.z;
+        r.u += f * (a.u + d * a.z);
+    }
+    if (b.m != -INFINITY) {
+        const float d = fmaxf(b.m - m, -150.f), f = exp_of(d);     // (0 beyond that, which a difference near the type's end must not turn into NaN)
+        r.z += f * b.z;
+        r.u += f * (b.u + d * b.z);
+    }
+    return r;
+}
+
+struct Part { Sums sums; int before, noted; u64 bound; };      // what a block of a row's cluster hands to the first one
+
+// Entries j0 .. j0 + VEC of a row, of which those in [lo, hi) count; others come back as -inf.
+template <typename T> struct Piece;
+template <> struct Piece<float> {
+    static constexpr int VEC = 4;
+    static __device__ __forceinline__ void load(const float* row, int j, float (&x)[4]) {
+        const float4 v = *reinterpret_cast<const float4*>(row + j);
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    }
+};
+template <> struct Piece<bf16> {
+    static constexpr int VEC = 8;
+    static __device__ __forceinline__ void load(const bf16* row, int j, float (&x)[8]) {
+        const uint4 v = *reinterpret_cast<const uint4*>(row + j);
+        const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+};
+
+// A round: the thread's LP_ROUND / VEC vectors, LP_THREADS vectors apart.  `row` starts on 16 bytes when `lead` entries before the row's first
+// are counted in (they lie outside [lo, hi)).
+template <typename T>
+__device__ __forceinline__ void load_round(const T* __restrict__ row, int at, int lo, int hi, float (&x)[LP_ROUND]) {
+    constexpr int VEC = Piece<T>::VEC;
+#pragma unroll
+    for (int u = 0; u < LP_ROUND / VEC; ++u) {
+        const int j = at + (u * LP_THREADS + (int)threadIdx.x) * VEC;
+        float v[VEC];
+        if (j >= lo && j + VEC <= hi) Piece<T>::load(row, j, v);
+        else {
+#pragma unroll
+            for (int c = 0; c < VEC; ++c) v[c] = j + c >= lo && j + c < hi ? to_float(row[j + c]) : -INFINITY;
+        }
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) x[u * VEC + c] = v[c];
+    }
+}
+template <typename T> __device__ __forceinline__ int index_in_round(int at, int e) {
+    constexpr int VEC = Piece<T>::VEC;
+    return at + ((e / VEC) * LP_THREADS + (int)threadIdx.x) * VEC + e % VEC;
+}
+
+// The keys in list[0..n) cut down to the `keep` largest, in order; all threads; `out` holds `keep` keys.
+__device__ __forceinline__ void select_largest(const u64* list, int n, int keep, u64* out) {
+    for (int i = threadIdx.x; i < n; i += LP_THREADS) {
+        const u64 mine = list[i];
+        int above = 0;
+        for (int j = 0; j < n; ++j) above += list[j] > mine;
+        if (above < keep) out[above] = mine;
+    }
+    __syncthreads();
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(float* __restrict__ logprobs, float* __restrict__ entropy,
+        int* __restrict__ ranks, int* __restrict__ top_ids, float* __restrict__ top_logprobs, const T* __restrict__ logits, long long stride,
+        const int* __restrict__ targets, int V, int top, int blocks, int* status) {
+    constexpr int VEC = Piece<T>::VEC;
+    __shared__ u64 list[TOP ? LP_ROOM : 1];
+    __shared__ u64 best[32], groups[TOP ? 32 : 1];
+    __shared__ u64 warp_best[TOP ? LP_THREADS : 1];
+    __shared__ u64 bound_s;
+    __shared__ int noted;
+    __shared__ Part part;
+    __shared__ Sums warp_sums[LP_WARPS];
+    __shared__ int warp_before[LP_WARPS];
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int r = (int)blockIdx.x / blocks, b = (int)blockIdx.x - r * blocks;
+    if (t == 0) {
+        noted = 0;
+        bound_s = 0;
+    }
+    pdl_trigger();
+    pdl_wait();
+    const T* row = logits + (long long)r * stride;
+    // indices from here on count from a 16-byte boundary at or before the row
+    const int lead = (int)(((uintptr_t)row & 15) / sizeof(T));
+    const T* base = row - lead;
+    const int target = targets[r];
+    const bool asked = (unsigned)target < (unsigned)V;
+    const float xt = asked ? to_float(row[target]) + 0.f : 0.f;
+    if (t == 0 && b == 0 && !asked && target != -1) zai_raise(status, ZAI_ST_TOKEN);
+    // this block's share: whole rounds' vectors, [lo, hi)
+    const int vectors = (V + lead + VEC - 1) / VEC, share = (vectors + blocks - 1) / blocks;
+    const int first = b * share * VEC;
+    const int lo = max(first, lead), hi = min(first + share * VEC, V + lead);
+    const int jt = asked ? target + lead : -1;                 // entries before it count when they are equal
+    // the next value above xt: x >= that is x > xt
+    const float above_xt = xt == INFINITY ? NAN : xt == 0.f ? __int_as_float(1) : __int_as_float(__float_as_int(xt) + (xt > 0.f ? 1 : -1));
+
+    Sums mine = {-INFINITY, 0.f, 0.f};
+    int before = 0;
+    u64 bound = 0;
+    float bound_x = -INFINITY;
+    float x[LP_ROUND], nx[LP_ROUND];
+    const int step = LP_THREADS * LP_ROUND;
+    load_round<T>(base, first, lo, hi, x);
+    for (int at = first; at < hi; at += step) {
+        if (at + step < hi) load_round<T>(base, at + step, lo, hi, nx);
+        float top_x = x[0];
+#pragma unroll
+        for (int e = 1; e < LP_ROUND; ++e) top_x = fmaxf(top_x, x[e]);
+        if (TOP) {
+            if (at == first) {                                 // (every block takes part, one without entries too: below)
+                u64 k = 0;
+#pragma unroll
+                for (int e = 0; e < LP_ROUND; ++e) {
+                    const int j = index_in_round<T>(at, e);
+                    if (j >= lo && j < hi) k = max(k, key_of(x[e], j - lead));
+                }
+                warp_best[t] = k;
+                __syncthreads();
+                if (warp == 0) {
+#pragma unroll
+                    for (int w = 1; w < LP_WARPS; ++w) k = max(k, warp_best[w * 32 + lane]);
+                    groups[lane] = k;
+                    __syncwarp();
+                    int above = 0;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) above += groups[i] > k || (groups[i] == k && i < lane);   // (groups without entries are equal)
+                    if (above == top - 1) bound_s = k;
+                }
+                __syncthreads();
+                bound = bound_s;
+                bound_x = fmaxf(value_of(bound), -INFINITY);    // (no bound, or one that is not a number: everything)
+            }
+            if (top_x >= bound_x || top_x != top_x) {
+#pragma unroll
+                for (int e = 0; e < LP_ROUND; ++e) {
+                    const int j = index_in_round<T>(at, e);
+                    const u64 k = key_of(x[e], j - lead);
+                    if (k >= bound && j >= lo && j < hi) {
+                        const int p = atomicAdd(&noted, 1);
+                        if (p < LP_ROOM) list[p] = k;
+                    }
+                }
+            }
+        }
+        if (top_x > mine.m) {
+            const Sums none = {top_x, 0.f, 0.f};
+            mine = joined(mine, none);
+        }
+        if (mine.m != -INFINITY) {
+#pragma unroll
+            for (int e = 0; e < LP_ROUND; ++e) {
+                const float d = x[e] - mine.m, w = exp_of(d);
+                mine.z += w;
+                mine.u += w * fmaxf(d, -150.f);                // (of -inf: 0, not 0 times infinity)
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < LP_ROUND; ++e)
+                if (x[e] != x[e]) mine = {0.f, NAN, NAN};      // (nothing else than -inf so far)
+        }
+#pragma unroll
+        for (int u = 0; u < LP_ROUND / VEC; ++u) {
+            const int j = index_in_round<T>(at, u * VEC);
+            if (jt < j || jt >= j + VEC) {
+                const float need = j < jt ? xt : above_xt;
+#pragma unroll
+                for (int c = 0; c < VEC; ++c) before += x[u * VEC + c] >= need;
+            } else {
+#pragma unroll
+                for (int c = 0; c < VEC; ++c) before += x[u * VEC + c] >= (j + c < jt ? xt : above_xt);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < LP_ROUND; ++e) x[e] = nx[e];
+    }
+    if (xt == -INFINITY && asked) {
+        // entries outside [lo, hi) came as -inf and were counted as equal ones before the token: counted again, by index
+        before = 0;
+        for (int j = lo + t; j < hi; j += LP_THREADS) {
+            const float v = to_float(base[j]);
+            before += v > xt || (v == xt && j < jt);
+        }
+    }
+    // the block's sums
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const Sums other = {__shfl_xor_sync(0xffffffffu, mine.m, o), __shfl_xor_sync(0xffffffffu, mine.z, o), __shfl_xor_sync(0xffffffffu, mine.u, o)};
+        mine = joined(mine, other);
+        before += __shfl_xor_sync(0xffffffffu, before, o);
+    }
+    if (lane == 0) {
+        warp_sums[warp] = mine;
+        warp_before[warp] = before;
+    }
+    __syncthreads();
+    if (TOP) {
+        if (noted > LP_ROOM) {
+            // more keys than there is room for: once more, a slice of at most LP_THREADS entries at a time, the list cut down when the next slice may not fit
+            __syncthreads();
+            if (t == 0) noted = 0;
+            __syncthreads();
+            for (int at = lo; at < hi; at += LP_THREADS) {
+                const int j = at + t;
+                if (j < hi) {
+                    const u64 k = key_of(to_float(base[j]), j - lead);
+                    if (k >= bound) list[atomicAdd(&noted, 1)] = k;
+                }
+                __syncthreads();
+                const int now = noted;
+                __syncthreads();
+                if (now > LP_ROOM - LP_THREADS) {
+                    select_largest(list, now, top, best);
+                    if (t < top) list[t] = best[t];
+                    if (t == 0) noted = top;
+                    bound = best[top - 1];
+                    __syncthreads();
+                }
+            }
+            if (t == 0) bound_s = bound;
+            __syncthreads();
+        }
+        if (blocks > 1 && noted > LP_PART) {
+            select_largest(list, noted, top, best);
+            if (t < top) list[t] = best[t];
+            if (t == 0) {
+                noted = top;
+                bound_s = best[top - 1];
+            }
+            __syncthreads();
+        }
+    }
+    if (warp == 0) {
+        Sums s = lane < LP_WARPS ? warp_sums[lane] : Sums{-INFINITY, 0.f, 0.f};
+        int n = lane < LP_WARPS ? warp_before[lane] : 0;
+#pragma unroll
+        for (int o = LP_WARPS / 2; o > 0; o >>= 1) {
+            const Sums other = {__shfl_xor_sync(0xffffffffu, s.m, o), __shfl_xor_sync(0xffffffffu, s.z, o), __shfl_xor_sync(0xffffffffu, s.u, o)};
+            s = joined(s, other);
+            n += __shfl_xor_sync(0xffffffffu, n, o);
+        }
+        if (lane == 0) part = {s, n, TOP ? noted : 0, bound_s};
+    }
+    __syncthreads();
+    Sums all = part.sums;
+    int rank = part.before, n = part.noted;
+    if (blocks > 1) {
+        cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        if (b == 0) {
+            all = {-INFINITY, 0.f, 0.f};
+            rank = 0;
+            u64 low = 0;
+            for (int i = 0; i < blocks; ++i) {                 // (in the blocks' order: the sums do not depend on who comes first)
+                const Part p = *cluster.map_shared_rank(&part, i);
+                all = joined(all, p.sums);
+                rank += p.before;
+                low = max(low, p.bound);                       // every block's bound is one of the row's
+            }
+            if (TOP) {
+                // the other blocks' keys at or above the highest bound, behind this block's own (at most LP_ROOM in all)
+                if (warp > 0 && warp < blocks) {
+                    const int count = cluster.map_shared_rank(&part, warp)->noted;
+                    const u64* theirs = cluster.map_shared_rank(list, warp);
+                    for (int i = lane; i < count; i += 32) {
+                        const u64 k = theirs[i];
+                        if (k >= low) list[atomicAdd(&noted, 1)] = k;
+                    }
+                }
+                __syncthreads();
+                n = noted;
+            }
+        }
+        cluster.sync();                                        // the other blocks' shared memory has been read
+        if (b != 0) return;
+    }
+    const float log_z = logf(all.z);
+    if (t == 0) {
+        logprobs[r] = asked ? xt - all.m - log_z : 0.f;
+        entropy[r] = log_z - all.u / all.z;
+        ranks[r] = asked ? rank : -1;
+    }
+    if (TOP) {
+        select_largest(list, n, top, best);
+        if (t < top) {
+            const u64 k = best[t];
+            top_ids[(size_t)r * top + t] = (int)~(unsigned)k;
+            top_logprobs[(size_t)r * top + t] = value_of(k) - all.m - log_z;
+        }
+    }
+}
+
+template <typename T>
+static int launch_logprobs(float* logprobs, float* entropy, int* ranks, int* top_ids, float* top_logprobs, const void* logits, long long stride,
+                           const int* targets, int R, int V, int top, int blocks, int* status, cudaStream_t stream) {
+    const auto kernel = top ? token_logprobs_kernel<T, true> : token_logprobs_kernel<T, false>;
+    static unsigned long long done[2] = {0, 0};
+    if (zai_first_on_device(&done[top > 0])) cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)R * blocks);
+    cfg.blockDim = dim3(LP_THREADS);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = blocks;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, logprobs, entropy, ranks, top_ids, top_logprobs, (const T*)logits, stride, targets, V, top, blocks,
+                                   status);
+}
+
+// `blocks` (a power of two up to 16): blocks that share a row; 0: as many as leave every block at least one round of the walk and fill the chip once.
+ZAI_API int zai_token_logprobs(float* logprobs, float* entropy, int* ranks, int* top_ids, float* top_logprobs, const void* logits, int dtype,
+                               long long stride, const int* targets, int R, int V, int top, int blocks, int sms, int* status,
+                               cudaStream_t stream) {
+    if (R < 1 || V < 1 || V > 0x7fffffff - 2 * LP_THREADS * LP_ROUND || R > 0x7fffffff / 16 || top < 0 || top > 32 || top > V || blocks < 0 || blocks > 16 ||
+        (blocks & (blocks - 1)))
+        return ZAI_BAD_SIZE;
+    if (blocks == 0)
+        for (blocks = 1; blocks < 16 && (long long)R * blocks * 2 <= 2 * sms && V / (blocks * 2) >= LP_THREADS * LP_ROUND / 2;) blocks *= 2;
+    ZAI_DISPATCH(dtype, return launch_logprobs<T>(logprobs, entropy, ranks, top_ids, top_logprobs, logits, stride, targets, R, V, top, blocks, status, stream));
+}

@@ -1,0 +1,660 @@
+// Attention of trees of drafted tokens.  Row i of a request's span sees the request's cached positions 0..ctx-1 and those rows j of
+// the span whose bit stands in its mask (its ancestors and itself, as a rule); with a window w > 0, of all these the ones whose position
+// is above the row's minus w:
+//
+//     o[i, h] = sum_j p_j v_j,  p = softmax over what i sees of scale q[i, h] . k_j         (nothing seen: zeros)
+//
+// Cached keys and values lie in the request's pages; the span's own are rows of k and v and enter no page before they are accepted.
+// A row's position is ctx plus its depth in the tree, so between ctx and ctx plus the span's rows.
+//
+// What bounds it: the cached keys and values, read once for all rows and query heads that share a key/value head.  So a tile of rows is
+// (row, query head) pairs of one key/value head, up to 128 of them, and the keys of a request are split over a cluster of up to 16
+// blocks whose parts are joined through distributed shared memory: no scratch in global memory, no counters, one launch, and an
+// order of the sums that depends on the sizes alone.
+//
+// Two kernels: bfloat16 heads of 32, 64, 96 and 128 on mma.sync, and a general one in 32-bit arithmetic for everything else.
+#include <cooperative_groups.h>
+#include "mma_helpers.cuh"
+namespace cg = cooperative_groups;
+
+#define MAX_SPLITS 16
+#define LOG2E 1.4426950408889634f
+
+struct TreeArgs {
+    void* out;
+    const void *q, *k, *v, *pages;
+    long long q_stride, k_stride, v_stride;                    // in elements
+    const int *table, *cu, *ctx, *positions;
+    const unsigned* mask;
+    int table_width, words, S, N, page_size, num_pages, H, G, D, window;
+    float scale;
+    int* status;
+};
+
+// The rows of one tile: span `s` of the step from row `first` on, `n` rows, `ctx` cached positions; the tile's pairs start at `pair0` of
+// the span's n * H / G.
+struct Tile { int s, first, n, ctx, pair0; };
+
+// The tile with this number when every span is cut into tiles of M pairs; all lanes of a warp.  s < 0: there is none.
+__device__ __forceinline__ Tile find_tile(const TreeArgs& a, int number, int M) {
+    const int lane = threadIdx.x & 31, group = a.H / a.G;
+    for (int at = 0; at < a.S; at += 32) {
+        const int s = at + lane;
+        int first = 0, n = 0;
+        if (s < a.S) {
+            first = a.cu[s];
+            n = a.cu[s + 1] - first;
+            if (n > 0 && (first < 0 || first + n > a.N)) {     // (rows outside the step: the span is passed over)
+                zai_raise(a.status, ZAI_ST_ROWS);
+                n = 0;
+            }
+        }
+        const int tiles = n > 0 ? (n * group + M - 1) / M : 0;
+        int upto = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        const unsigned here = __ballot_sync(0xffffffffu, number < upto);
+        if (here) {
+            const int w = __ffs(here) - 1;
+            Tile t;
+            t.s = at + w;
+            t.first = __shfl_sync(0xffffffffu, first, w);
+            t.n = __shfl_sync(0xffffffffu, n, w);
+            t.pair0 = (number - __shfl_sync(0xffffffffu, upto - tiles, w)) * M;
+            t.ctx = max(a.ctx[t.s], 0);
+            return t;
+        }
+        number -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return {-1, 0, 0, 0, 0};
+}
+
+// Does row `node` of the tile's span see row `other`?
+__device__ __forceinline__ bool sees_node(const TreeArgs& a, const Tile& t, int node, int pos, int other) {
+    if (other >= t.n || (other >> 5) >= a.words) return false;
+    if (!(a.mask[(size_t)(t.first + node) * a.words + (other >> 5)] >> (other & 31) & 1u)) return false;
+    return a.window <= 0 || a.positions[t.first + other] > pos - a.window;
+}
+
+// ---------------------------------------------------------------------------------------------------- the general kernel
+// A block owns 16 pairs, a warp four of them; per tile of 32 keys a lane computes its key's scores with the warp's pairs, the weights go
+// through shared memory, and the lanes share out the columns.  Keys and values are converted to 32 bits on their way to shared memory.
+#define GEN_PAIRS 16
+#define GEN_KEYS 32
+#define GEN_THREADS 128
+
+// The sum p * v of a tile's keys; GUARD: a key that has no weight stays out whatever its value is.
+template <int COLS, bool GUARD>
+__device__ __forceinline__ void add_values(float (&o)[4][COLS], const float* p, const float* v, int D, int lane) {
+    for (int j = 0; j < GEN_KEYS; ++j) {
+        const float4 w = *reinterpret_cast<const float4*>(p + 4 * j);
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) {
+            const int d = lane + 32 * c;
+            const float x = d < D ? v[j * D + d] : 0.f;
+            if (!GUARD || w.x != 0.f) o[0][c] = fmaf(w.x, x, o[0][c]);
+            if (!GUARD || w.y != 0.f) o[1][c] = fmaf(w.y, x, o[1][c]);
+            if (!GUARD || w.z != 0.f) o[2][c] = fmaf(w.z, x, o[2][c]);
+            if (!GUARD || w.w != 0.f) o[3][c] = fmaf(w.w, x, o[3][c]);
+        }
+    }
+}
+
+template <typename T, int COLS>
+__global__ void __launch_bounds__(GEN_THREADS) tree_attention_general_kernel(const TreeArgs a, int splits) {
+    extern __shared__ float sm[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = a.D, group = a.H / a.G, head = blockIdx.y, rank = blockIdx.x % splits;
+    const int D4 = (D + 3) & ~3, KS = D4 + 4;                  // a key's row: four floats further than its length, so that lanes meet no bank twice
+    float* qs = sm;                                            // [16][D4]
+    float* ks = qs + GEN_PAIRS * D4;                           // [32][KS]
+    float* vs = ks + GEN_KEYS * KS;                            // [32][D]
+    float* ps = vs + GEN_KEYS * D4;                            // [4 warps][32 keys][4 pairs]
+    float* ml = ps + GEN_PAIRS * GEN_KEYS;                     // [16][2]
+    pdl_trigger();
+    pdl_wait();
+    const Tile t = find_tile(a, blockIdx.x / splits, GEN_PAIRS);
+    if (t.s < 0) return;                                       // (the whole cluster's)
+    const int pairs = min(t.n * group - t.pair0, GEN_PAIRS);
+    for (int e = threadIdx.x; e < GEN_PAIRS * D4; e += GEN_THREADS) {
+        const int r = e / D4, d = e - r * D4, p = t.pair0 + r;
+        qs[e] = r < pairs && d < D ? to_float(((const T*)a.q)[(long long)(t.first + p / group) * a.q_stride + (head * group + p % group) * D + d]) : 0.f;
+    }
+    int node[4], pos[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = warp * 4 + i;
+        node[i] = r < pairs ? (t.pair0 + r) / group : -1;
+        pos[i] = node[i] >= 0 && a.window > 0 ? a.positions[t.first + node[i]] : 0;
+    }
+    const int first_key = a.window > 0 ? max(t.ctx - a.window + 1, 0) : 0;
+    const int tile0 = first_key / GEN_KEYS, cached = max((t.ctx + GEN_KEYS - 1) / GEN_KEYS - tile0, 0), total = cached + (t.n + GEN_KEYS - 1) / GEN_KEYS;
+    const int from = (int)((long long)total * rank / splits), upto = (int)((long long)total * (rank + 1) / splits);
+    const ZaiTableRow table = {a.table + (size_t)t.s * a.table_width, a.table_width, a.num_pages, a.status};
+    float o[4][COLS], m[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) o[i][c] = 0.f;
+    }
+    for (int it = from; it < upto; ++it) {
+        const bool nodes = it >= cached;
+        const int key0 = nodes ? (it - cached) * GEN_KEYS : (tile0 + it) * GEN_KEYS;
+        __syncthreads();                                       // (the tile before has been used)
+        bool odd = false;
+        for (int j = warp; j < GEN_KEYS; j += GEN_THREADS / 32) {
+            const T *kp = nullptr, *vp = nullptr;
+            const int key = key0 + j;
+            if (nodes) {
+                if (key < t.n) {
+                    kp = (const T*)a.k + (long long)(t.first + key) * a.k_stride + head * D;
+                    vp = (const T*)a.v + (long long)(t.first + key) * a.v_stride + head * D;
+                }
+            } else if (key < t.ctx && key >= first_key) {
+                const int idx = key / a.page_size;
+                kp = (const T*)a.pages + (((long long)table.page(idx) * 2 * a.G + head) * a.page_size + (key - idx * a.page_size)) * D;
+                vp = kp + (long long)a.G * a.page_size * D;
+            }
+            for (int d = lane; d < D4; d += 32) {
+                ks[j * KS + d] = kp && d < D ? to_float(kp[d]) : 0.f;
+                if (d < D) {
+                    const float x = vp ? to_float(vp[d]) : 0.f;
+                    odd |= !(fabsf(x) < INFINITY);
+                    vs[j * D + d] = x;
+                }
+            }
+        }
+        odd = __syncthreads_or(odd);
+        // scores: this lane's key with the warp's pairs
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        const float* kr = ks + lane * KS;
+        const float* qr = qs + warp * 4 * D4;
+        for (int d = 0; d < D4; d += 4) {
+            const float4 k4 = *reinterpret_cast<const float4*>(kr + d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float4 q4 = *reinterpret_cast<const float4*>(qr + i * D4 + d);
+                s[i] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[i]))));
+            }
+        }
+        float4 w;
+        float* wp = &w.x;
+        const int key = key0 + lane;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool seen = node[i] >= 0 && (nodes ? sees_node(a, t, node[i], pos[i], key)
+                                                     : key < t.ctx && (a.window <= 0 || key > pos[i] - a.window));
+            const float x = seen ? s[i] * a.scale : -INFINITY;
+            const float top = fmaxf(m[i], warp_max(x));
+            const float keep = top == -INFINITY ? 1.f : expf(m[i] - top);
+            const float p = seen ? expf(x - top) : 0.f;
+            l[i] = l[i] * keep + p;                            // (a lane's own keys; added up at the end)
+            m[i] = top;
+            wp[i] = p;
+#pragma unroll
+            for (int c = 0; c < COLS; ++c) o[i][c] *= keep;
+        }
+        float* mine = ps + warp * GEN_KEYS * 4;
+        __syncwarp();
+        *reinterpret_cast<float4*>(mine + 4 * lane) = w;
+        __syncwarp();
+        if (odd) add_values<COLS, true>(o, mine, vs, D, lane);
+        else add_values<COLS, false>(o, mine, vs, D, lane);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) l[i] = warp_sum(l[i]);
+    T* out = (T*)a.out;
+    if (splits == 1) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (node[i] < 0) continue;
+            const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+            T* row = out + ((long long)(t.first + node[i]) * a.H + head * group + (t.pair0 + warp * 4 + i) % group) * D;
+#pragma unroll
+            for (int c = 0; c < COLS; ++c)
+                if (lane + 32 * c < D) row[lane + 32 * c] = from_float<T>(l[i] == 0.f ? 0.f : o[i][c] * inv);
+        }
+        return;
+    }
+    // the blocks' parts: O in shared memory (over the tiles), references and sums behind it; every block joins some of the pairs
+    __syncthreads();
+    float* po = ks;                                            // [16][D]
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = warp * 4 + i;
+#pragma unroll
+        for (int c = 0; c < COLS; ++c)
+            if (lane + 32 * c < D) po[r * D + lane + 32 * c] = o[i][c];
+        if (lane == 0) {
+            ml[2 * r] = m[i];
+            ml[2 * r + 1] = l[i];
+        }
+    }
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    for (int r = rank + warp * splits; r < pairs; r += splits * (GEN_THREADS / 32)) {
+        float top = -INFINITY;
+        for (int i = 0; i < splits; ++i) top = fmaxf(top, cluster.map_shared_rank(ml, i)[2 * r]);
+        float sum = 0.f, x[COLS];
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) x[c] = 0.f;
+        for (int i = 0; i < splits; ++i) {
+            const float* theirs = cluster.map_shared_rank(ml, i);
+            const float part = theirs[2 * r + 1];
+            if (part == 0.f) continue;                         // (a block that saw nothing of this pair)
+            const float f = expf(theirs[2 * r] - top);
+            const float* vals = cluster.map_shared_rank(po, i) + r * D;
+            sum += f * part;
+#pragma unroll
+            for (int c = 0; c < COLS; ++c)
+                if (lane + 32 * c < D) x[c] += f * vals[lane + 32 * c];
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const int p = t.pair0 + r;
+        T* row = out + ((long long)(t.first + p / group) * a.H + head * group + p % group) * D;
+#pragma unroll
+        for (int c = 0; c < COLS; ++c)
+            if (lane + 32 * c < D) row[lane + 32 * c] = from_float<T>(sum == 0.f ? 0.f : x[c] * inv);
+    }
+    cluster.sync();                                            // (the parts have been read)
+}
+
+// ---------------------------------------------------------------------------------------------------- bfloat16 on mma.sync
+// A block owns 16 WM pairs; its warps are WM rows of 16 pairs times WN shares of every tile of 64 keys, each share with a maximum,
+// a sum and an O of its own (joined with those of the cluster's other blocks at the end).  Keys and values come by cp.async, STAGES tiles
+// in a ring; where a tile's 64 keys lie is looked up a turn before its copies are issued, by one thread a key.  Q stays in registers,
+// scores go from the accumulators into the second product's operand without leaving them.  Weights are rounded to bfloat16 there, as
+// the values are; their sum is taken before the rounding, in 32 bits.
+#define KEYS 64
+
+template <int D, int WM, int WN, int STAGES> struct MmaShape {
+    static constexpr int THREADS = 32 * WM * WN, PAIRS = 16 * WM, ROW = D + 8, STAGE = 2 * KEYS * ROW, KW = KEYS / WN, O_ROW = D + 8;
+    static constexpr size_t RING = sizeof(bf16) * STAGES * STAGE;
+    static constexpr size_t JOIN = sizeof(float) * WN * PAIRS * O_ROW;
+    static constexpr size_t SMEM = (RING > JOIN ? RING : JOIN) + sizeof(void*) * 4 * KEYS + sizeof(float) * 2 * WN * PAIRS;
+};
+
+template <int D, int WM, int WN, int STAGES>
+__global__ void __launch_bounds__(32 * WM * WN) tree_attention_mma_kernel(const TreeArgs a, int splits) {
+    using Shape = MmaShape<D, WM, WN, STAGES>;
+    constexpr int THREADS = Shape::THREADS, PAIRS = Shape::PAIRS, ROW = Shape::ROW, KW = Shape::KW, NT = KW / 8, O_ROW = Shape::O_ROW;
+    constexpr int CHUNKS = D / 8;                              // pieces of 16 bytes a key
+    extern __shared__ __align__(16) char smem[];
+    bf16* ring = reinterpret_cast<bf16*>(smem);
+    const bf16** where = reinterpret_cast<const bf16**>(smem + (Shape::RING > Shape::JOIN ? Shape::RING : Shape::JOIN));     // [2][KEYS][key, value]
+    float* ml = reinterpret_cast<float*>(where + 4 * KEYS);    // [WN][PAIRS][2]
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wm = warp % WM, wn = warp / WM, head = blockIdx.y, rank = blockIdx.x % splits;
+    const int group = a.H / a.G, g = lane >> 2, q4 = lane & 3;
+    pdl_trigger();
+    pdl_wait();
+    const Tile t = find_tile(a, blockIdx.x / splits, PAIRS);
+    if (t.s < 0) return;                                       // (the whole cluster's)
+    const int pairs = min(t.n * group - t.pair0, PAIRS);
+    const int first_key = a.window > 0 ? max(t.ctx - a.window + 1, 0) : 0;
+    const int tile0 = first_key / KEYS, cached = max((t.ctx + KEYS - 1) / KEYS - tile0, 0), total = cached + (t.n + KEYS - 1) / KEYS;
+    const int from = (int)((long long)total * rank / splits), upto = (int)((long long)total * (rank + 1) / splits);
+    const ZaiTableRow table = {a.table + (size_t)t.s * a.table_width, a.table_width, a.num_pages, a.status};
+
+    auto look_up = [&](int it) {                               // where tile `it`'s keys lie, by the first KEYS threads
+        if ((int)threadIdx.x >= KEYS || it >= upto) return;
+        const int j = threadIdx.x;
+        const bf16 *kp = nullptr, *vp = nullptr;
+        if (it >= cached) {
+            const int key = (it - cached) * KEYS + j;
+            if (key < t.n) {
+                kp = (const bf16*)a.k + (long long)(t.first + key) * a.k_stride + head * D;
+                vp = (const bf16*)a.v + (long long)(t.first + key) * a.v_stride + head * D;
+            }
+        } else {
+            const int key = (tile0 + it) * KEYS + j;
+            if (key < t.ctx && key >= first_key) {
+                const int idx = key / a.page_size;
+                kp = (const bf16*)a.pages + (((long long)table.page(idx) * 2 * a.G + head) * a.page_size + (key - idx * a.page_size)) * D;
+                vp = kp + (long long)a.G * a.page_size * D;
+            }
+        }
+        const bf16** w = where + ((it & 1) * KEYS + j) * 2;
+        w[0] = kp;
+        w[1] = vp;
+    };
+    auto issue = [&](int it) {                                 // tile `it`'s copies; keys that are not there become zeros
+        if (it < upto) {
+            bf16* ks = ring + (it % STAGES) * Shape::STAGE;
+#pragma unroll
+            for (int e = threadIdx.x; e < KEYS * CHUNKS; e += THREADS) {
+                const int j = e / CHUNKS, c = e - j * CHUNKS;
+                const bf16* const* w = where + ((it & 1) * KEYS + j) * 2;
+                const bf16 *kp = w[0], *vp = w[1];
+                cp_async16(ks + j * ROW + c * 8, kp ? kp + c * 8 : (const bf16*)a.pages, kp != nullptr);
+                cp_async16(ks + (KEYS + j) * ROW + c * 8, vp ? vp + c * 8 : (const bf16*)a.pages, vp != nullptr);
+            }
+        }
+        cp_async_commit();
+    };
+
+    // this lane's two pairs: g and g + 8 of the warp's 16
+    int node[2], pos[2];
+    uint32_t qf[D / 16][4];
+    {
+        const bf16* qr[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = wm * 16 + g + 8 * i, p = t.pair0 + r;
+            node[i] = r < pairs ? p / group : -1;
+            pos[i] = node[i] >= 0 && a.window > 0 ? a.positions[t.first + node[i]] : 0;
+            qr[i] = node[i] >= 0 ? (const bf16*)a.q + (long long)(t.first + node[i]) * a.q_stride + (head * group + p % group) * D + 2 * q4 : nullptr;
+        }
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                qf[kk][i] = qr[i & 1] ? *reinterpret_cast<const uint32_t*>(qr[i & 1] + kk * 16 + (i >> 1) * 8) : 0u;
+    }
+    const bool idle = wm * 16 >= pairs;                        // a warp without pairs brings keys in and computes nothing
+    for (int it = from; it < from + STAGES - 1; ++it) {
+        look_up(it);
+        __syncthreads();
+        issue(it);
+    }
+    look_up(from + STAGES - 1);
+
+    float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < D / 8; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d][e] = 0.f;
+    const float scale = a.scale * LOG2E;
+    for (int it = from; it < upto; ++it) {
+        cp_async_wait<STAGES - 2>();
+        __syncthreads();
+        issue(it + STAGES - 1);
+        look_up(it + STAGES);
+        if (idle) continue;
+        const bf16* ks = ring + (it % STAGES) * Shape::STAGE + wn * KW * ROW;
+        const bf16* vs = ks + KEYS * ROW;
+        float s[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+            for (int n = 0; n < NT; n += 2) {
+                uint32_t b[4];
+                ldmatrix_x4(b, ks + (n * 8 + (lane & 7) + ((lane & 16) >> 1)) * ROW + kk * 16 + (lane & 8));
+                mma_bf16(s[n], qf[kk], b[0], b[1]);
+                mma_bf16(s[n + 1], qf[kk], b[2], b[3]);
+            }
+        const bool nodes = it >= cached;
+        const int key0 = (nodes ? it - cached : tile0 + it) * KEYS;
+        // every pair sees all keys of the tile?  (positions lie between ctx and ctx + n)
+        const bool whole = !nodes && key0 + KEYS <= t.ctx && (a.window <= 0 || key0 > t.ctx + t.n - 1 - a.window);
+        bool odd = false;
+        if (!whole) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = e >> 1, key = key0 + wn * KW + n * 8 + 2 * q4 + (e & 1);
+                    const bool seen = node[i] >= 0 && (nodes ? sees_node(a, t, node[i], pos[i], key)
+                                                             : key < t.ctx && (a.window <= 0 || key > pos[i] - a.window));
+                    if (!seen) s[n][e] = -INFINITY;
+                }
+            // values that are not finite: they must not reach the pairs that do not see them as 0 times NaN
+            uint32_t bad = 0;
+            for (int e = lane; e < KW * CHUNKS; e += 32) {
+                const int j = e / CHUNKS;
+                const uint4 x = *reinterpret_cast<const uint4*>(vs + j * ROW + (e - j * CHUNKS) * 8);
+                bad |= not_finite_pair(x.x) | not_finite_pair(x.y) | not_finite_pair(x.z) | not_finite_pair(x.w);
+            }
+            odd = __any_sync(0xffffffffu, bad != 0);
+        }
+        // the running maximum, in units of the exponent
+        float top[2] = {m[0], m[1]};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            top[0] = fmaxf(top[0], fmaxf(s[n][0], s[n][1]) * scale);
+            top[1] = fmaxf(top[1], fmaxf(s[n][2], s[n][3]) * scale);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+            top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+        }
+        if (__any_sync(0xffffffffu, top[0] != m[0] || top[1] != m[1])) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float keep = top[i] == -INFINITY ? 1.f : fast_exp2(m[i] - top[i]);
+                m[i] = top[i];
+                l[i] *= keep;
+#pragma unroll
+                for (int d = 0; d < D / 8; ++d) {
+                    o[d][2 * i] *= keep;
+                    o[d][2 * i + 1] *= keep;
+                }
+            }
+        }
+        // weights; a pair that has seen nothing yet takes 0 as its reference, so that masked scores weigh 0
+        const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+        uint32_t pf[NT / 2][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float p[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                p[e] = fast_exp2(fmaf(s[n][e], scale, -ref[e >> 1]));
+                l[e >> 1] += p[e];
+            }
+            pf[n / 2][(n & 1) * 2] = pack_bf16(p[0], p[1]);
+            pf[n / 2][(n & 1) * 2 + 1] = pack_bf16(p[2], p[3]);
+        }
+        if (!odd) {
+#pragma unroll
+            for (int kk = 0; kk < NT / 2; ++kk)
+#pragma unroll
+                for (int d = 0; d < D / 8; d += 2) {
+                    uint32_t b[4];
+                    ldmatrix_x4_trans(b, vs + (kk * 16 + (lane & 15)) * ROW + d * 8 + ((lane & 16) >> 1));
+                    mma_bf16(o[d], pf[kk], b[0], b[1]);
+                    mma_bf16(o[d + 1], pf[kk], b[2], b[3]);
+                }
+        } else {
+            // the product without what is not finite, and a count of how many such values a pair gives weight to: those columns become NaN
+#pragma unroll
+            for (int d = 0; d < D / 8; d += 2) {
+                float hit[2][4] = {};
+#pragma unroll
+                for (int kk = 0; kk < NT / 2; ++kk) {
+                    uint32_t b[4], f[4], w[4];
+                    ldmatrix_x4_trans(b, vs + (kk * 16 + (lane & 15)) * ROW + d * 8 + ((lane & 16) >> 1));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t mark = not_finite_pair(b[i]) >> 15;             // 1 in the low bit of each half
+                        f[i] = mark * 0x3f80u;                                         // one
+                        b[i] &= ~(mark * 0xffffu);
+                        w[i] = ((pf[kk][i] & 0x7fffu) ? 0x3f80u : 0u) | ((pf[kk][i] & 0x7fff0000u) ? 0x3f800000u : 0u);
+                    }
+                    mma_bf16(o[d], pf[kk], b[0], b[1]);
+                    mma_bf16(o[d + 1], pf[kk], b[2], b[3]);
+                    mma_bf16(hit[0], w, f[0], f[1]);
+                    mma_bf16(hit[1], w, f[2], f[3]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (hit[0][e] > 0.f) o[d][e] = NAN;
+                    if (hit[1][e] > 0.f) o[d + 1][e] = NAN;
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    }
+    bf16* out = (bf16*)a.out;
+    if (WN == 1 && splits == 1) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (node[i] < 0) continue;
+            const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+            bf16* row = out + ((long long)(t.first + node[i]) * a.H + head * group + (t.pair0 + wm * 16 + g + 8 * i) % group) * D + 2 * q4;
+#pragma unroll
+            for (int d = 0; d < D / 8; ++d)
+                *reinterpret_cast<uint32_t*>(row + d * 8) = pack_bf16(o[d][2 * i] * inv, o[d][2 * i + 1] * inv);
+        }
+        cp_async_wait<0>();
+        return;
+    }
+    // the parts: WN of each block of the cluster, in shared memory over the ring; every block joins some of the pairs
+    cp_async_wait<0>();
+    __syncthreads();
+    float* po = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = wn * PAIRS + wm * 16 + g + 8 * i;
+#pragma unroll
+        for (int d = 0; d < D / 8; ++d) *reinterpret_cast<float2*>(po + r * O_ROW + d * 8 + 2 * q4) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
+        if (q4 == 0) {
+            ml[2 * r] = m[i];
+            ml[2 * r + 1] = l[i];
+        }
+    }
+    cg::cluster_group cluster = cg::this_cluster();
+    if (splits > 1) cluster.sync();
+    else __syncthreads();
+    constexpr int QUADS = D / 4;
+    const int mine = (pairs - rank + splits - 1) / splits;     // pairs rank, rank + splits, ...
+    for (int e = threadIdx.x; e < mine * QUADS; e += THREADS) {
+        const int r = rank + (e / QUADS) * splits, c = (e % QUADS) * 4;
+        float top = -INFINITY;
+#pragma unroll 4
+        for (int i = 0; i < splits * WN; ++i) {
+            const float* theirs = splits > 1 ? cluster.map_shared_rank(ml, i / WN) : ml;
+            top = fmaxf(top, theirs[2 * ((i % WN) * PAIRS + r)]);
+        }
+        float sum = 0.f;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int i = 0; i < splits * WN; ++i) {
+            const float* theirs = splits > 1 ? cluster.map_shared_rank(ml, i / WN) : ml;
+            const float* vals = splits > 1 ? cluster.map_shared_rank(po, i / WN) : po;
+            const int at = (i % WN) * PAIRS + r;
+            const float2 its = *reinterpret_cast<const float2*>(theirs + 2 * at);
+            const float4 v = *reinterpret_cast<const float4*>(vals + at * O_ROW + c);
+            if (its.y == 0.f) continue;                        // (a part that saw nothing of this pair)
+            const float f = fast_exp2(its.x - top);
+            sum = fmaf(f, its.y, sum);
+            x.x = fmaf(f, v.x, x.x);
+            x.y = fmaf(f, v.y, x.y);
+            x.z = fmaf(f, v.z, x.z);
+            x.w = fmaf(f, v.w, x.w);
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const int p = t.pair0 + r;
+        bf16* row = out + ((long long)(t.first + p / group) * a.H + head * group + p % group) * D + c;
+        uint2 w;
+        w.x = pack_bf16(x.x * inv, x.y * inv);
+        w.y = pack_bf16(x.z * inv, x.w * inv);
+        *reinterpret_cast<uint2*>(row) = w;
+    }
+    if (splits > 1) cluster.sync();                            // (the parts have been read)
+}
+
+// ---------------------------------------------------------------------------------------------------- launching
+template <typename... K>
+static int launch_cluster(void (*kernel)(K...), unsigned long long* done, dim3 grid, int threads, size_t smem, int splits, cudaStream_t stream,
+                          const TreeArgs& a) {
+    if (zai_first_on_device(done)) {
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = splits;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, a, splits);
+}
+
+template <typename T, int COLS>
+static int launch_general(const TreeArgs& a, int tiles, int splits, cudaStream_t stream) {
+    static unsigned long long done = 0;
+    const int D4 = (a.D + 3) & ~3;
+    const size_t smem = sizeof(float) * ((size_t)GEN_PAIRS * D4 + GEN_KEYS * (D4 + 4) + GEN_KEYS * D4 + GEN_PAIRS * GEN_KEYS + 2 * GEN_PAIRS);
+    return launch_cluster(tree_attention_general_kernel<T, COLS>, &done, dim3((unsigned)splits * tiles, a.G), GEN_THREADS, smem, splits, stream, a);
+}
+
+// Pairs of (row, query head) a block of the general kernel owns.
+ZAI_API int zai_tree_attention_general_pairs() { return GEN_PAIRS; }
+
+ZAI_API int zai_tree_attention_general(void* out, const void* q, long long q_stride, const void* k, long long k_stride, const void* v, long long v_stride,
+                                       const void* pages, int dtype, const int* table, int table_width, const int* cu, const int* ctx, const int* positions,
+                                       const int* mask, int words, int S, int N, int tiles, int splits, int page_size, int num_pages, int H, int G, int D,
+                                       float scale, int window, int* status, cudaStream_t stream) {
+    if (S < 1 || N < 1 || tiles < 1 || tiles > 0x7ffffff || splits < 1 || splits > MAX_SPLITS || page_size < 1 || num_pages < 1 || G < 1 || H % G || G > 65535 ||
+        D < 1 || D > 512 || words < 1 || table_width < 1 || (long long)N * (H / G) > 0x3fffffff)
+        return ZAI_BAD_SIZE;
+    const TreeArgs a = {out, q, k, v, pages, q_stride, k_stride, v_stride, table, cu, ctx, positions, (const unsigned*)mask, table_width, words, S, N,
+                        page_size, num_pages, H, G, D, window, scale, status};
+    ZAI_DISPATCH(dtype, {
+        if (D <= 32) return launch_general<T, 1>(a, tiles, splits, stream);
+        if (D <= 64) return launch_general<T, 2>(a, tiles, splits, stream);
+        if (D <= 128) return launch_general<T, 4>(a, tiles, splits, stream);
+        if (D <= 256) return launch_general<T, 8>(a, tiles, splits, stream);
+        return launch_general<T, 16>(a, tiles, splits, stream);
+    });
+}
+
+template <int D, int WM, int WN, int STAGES> static int launch_mma(const TreeArgs& a, int tiles, int splits, cudaStream_t stream) {
+    using Shape = MmaShape<D, WM, WN, STAGES>;
+    static_assert(Shape::SMEM <= 227 * 1024, "the ring does not fit");
+    static unsigned long long done = 0;
+    return launch_cluster(tree_attention_mma_kernel<D, WM, WN, STAGES>, &done, dim3((unsigned)splits * tiles, a.G), Shape::THREADS, Shape::SMEM, splits,
+                          stream, a);
+}
+template <int D> static int launch_mma_pairs(const TreeArgs& a, int pairs, int tiles, int splits, cudaStream_t stream) {
+    if (pairs == 16) return launch_mma<D, 1, 4, 3>(a, tiles, splits, stream);
+    if (pairs == 32) return launch_mma<D, 2, 2, 3>(a, tiles, splits, stream);
+    if (pairs == 64) return launch_mma<D, 4, 1, 3>(a, tiles, splits, stream);
+    if (pairs == 128) return launch_mma<D, 8, 1, 3>(a, tiles, splits, stream);
+    return ZAI_BAD_SIZE;
+}
+
+ZAI_API int zai_tree_attention_mma_supports(int D) { return D == 32 || D == 64 || D == 96 || D == 128; }
+
+// bfloat16; `pairs` (16, 32, 64 or 128): pairs of (row, query head) a block owns.  q starts on 4 bytes and has even row strides; keys and values,
+// of the pages and of the rows, start on 16 bytes.
+ZAI_API int zai_tree_attention_mma(void* out, const void* q, long long q_stride, const void* k, long long k_stride, const void* v, long long v_stride,
+                                   const void* pages, const int* table, int table_width, const int* cu, const int* ctx, const int* positions,
+                                   const int* mask, int words, int S, int N, int pairs, int tiles, int splits, int page_size, int num_pages, int H, int G,
+                                   int D, float scale, int window, int* status, cudaStream_t stream) {
+    if (S < 1 || N < 1 || tiles < 1 || tiles > 0x7ffffff || splits < 1 || splits > MAX_SPLITS || page_size < 1 || num_pages < 1 || G < 1 || H % G ||
+        G > 65535 || words < 1 || table_width < 1 || (long long)N * (H / G) > 0x3fffffff)
+        return ZAI_BAD_SIZE;
+    if ((((uintptr_t)k | (uintptr_t)v | (uintptr_t)pages) & 15) || ((k_stride | v_stride) & 7) || ((uintptr_t)q & 3) || (q_stride & 1) || ((uintptr_t)out & 7))
+        return ZAI_BAD_SIZE;
+    const TreeArgs a = {out, q, k, v, pages, q_stride, k_stride, v_stride, table, cu, ctx, positions, (const unsigned*)mask, table_width, words, S, N,
+                        page_size, num_pages, H, G, D, window, scale, status};
+    switch (D) {
+        case 32: return launch_mma_pairs<32>(a, pairs, tiles, splits, stream);
+        case 64: return launch_mma_pairs<64>(a, pairs, tiles, splits, stream);
+        case 96: return launch_mma_pairs<96>(a, pairs, tiles, splits, stream);
+        case 128: return launch_mma_pairs<128>(a, pairs, tiles, splits, stream);
+    }
+    return ZAI_BAD_SIZE;
+}

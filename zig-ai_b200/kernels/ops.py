@@ -14,6 +14,7 @@ import os
 import sys
 import weakref
 from ctypes import c_float, c_int, c_void_p
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -23,7 +24,7 @@ from . import build
 device_type = "cuda"
 
 _F32, _BF16 = 0, 1
-_P, _I, _F = c_void_p, c_int, c_float
+_P, _I, _F, _L = c_void_p, c_int, c_float, ctypes.c_longlong
 
 _SIGNATURES = {
     "embed": {
@@ -167,6 +168,20 @@ _SIGNATURES = {
         "zai_prefill_attention_tc_shaped_splits": [_I, _I, _I, _I],
         "zai_prefill_attention_tc_max_bias": [],
     },
+    "drafts": {
+        "zai_step_layout": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
+        "zai_accept_drafts": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P],
+        "zai_commit_drafts": [_P, _P, _P, _L, _L, _L, _L, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
+    },
+    "tree_attention": {
+        "zai_tree_attention_general_pairs": [],
+        "zai_tree_attention_general": [_P, _P, _L, _P, _L, _P, _L, _P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I,
+                                       _F, _I, _P, _P],
+        "zai_tree_attention_mma_supports": [_I],
+        "zai_tree_attention_mma": [_P, _P, _L, _P, _L, _P, _L, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I,
+                                   _F, _I, _P, _P],
+    },
+    "logprobs": {"zai_token_logprobs": [_P, _P, _P, _P, _P, _P, _I, _L, _P, _I, _I, _I, _I, _I, _P, _P]},
     "sampling": {
         "zai_argmax": [_P, _P, _I, _I, _P, _P],
         "zai_repetition_penalty": [_P, _P, _P, _P, _P, _I, _I, _P],
@@ -601,7 +616,8 @@ USE_TC_GEMM = os.environ.get("ZAI_TC_GEMM", "0") == "1"
 # with them and throws the step away if it is not zero.
 STATUS_BITS = {1: "a bounded wait inside a kernel ran out", 2: "a token id outside the vocabulary",
                4: "a block-table entry outside the page pool", 8: "a state slot outside the slots",
-               16: "a position outside its request's block-table row"}
+               16: "a position outside its request's block-table row", 32: "spans of more rows than the step has, or a row outside it",
+               64: "a drafted row whose parent is not before it, or a tree of too many rows"}
 _status = {}
 
 
@@ -1273,6 +1289,223 @@ def sample(logits, temperature, top_k, top_p, u, with_status=False):
     _check(_fn("sampling", "zai_sample")(_ptr(out), _ptr(logits), _ptr(temperature), _ptr(top_k), _ptr(top_p),
                                          _ptr(u), R, V, _status_ptr(logits.device) if with_status else None, _stream()), "sample")
     return out
+
+
+class TokenLogprobs(NamedTuple):
+    """What `token_logprobs` returns, a row per row of logits."""
+    logprobs: torch.Tensor                  # [R] 32-bit: of the given tokens
+    entropy: torch.Tensor                   # [R] 32-bit, in nats
+    ranks: torch.Tensor                     # [R] int32: how many tokens stand before the given one
+    top_ids: torch.Tensor                   # [R, top] int32: the likeliest tokens, in order
+    top_logprobs: torch.Tensor              # [R, top] 32-bit
+
+
+@_timed("sampling")
+def token_logprobs(logits, tokens, top=0, blocks=0):
+    """Log probabilities of given tokens (int32 [R]) under logits [R, V] (32-bit or bfloat16; rows may lie apart), the entropy of
+    every row, the tokens' ranks (0: the likeliest; equal logits by the lower id) and the `top` (at most 32) likeliest tokens
+    with theirs.  A token of -1 stands for none: log probability 0, rank -1.  Logits of -inf are tokens that cannot come; a row
+    with a NaN or +inf, or of -inf alone, has NaNs.  `blocks`: how many blocks share a row (0: by the sizes)."""
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise KernelError("token_logprobs: logits are rows [R, V]")
+    R, V = logits.shape
+    top = int(top)
+    if not logits.is_cuda or logits.stride(1) != 1 and V > 1 or logits.stride(0) < V and R > 1:
+        raise KernelError("token_logprobs: logits are rows of contiguous values on a CUDA device")
+    if tokens.dtype != torch.int32 or tokens.shape != (R,) or not tokens.is_contiguous() or tokens.device != logits.device:
+        raise KernelError("token_logprobs: the tokens are int32, one for each row of logits, on the logits' device")
+    if not 0 <= top <= min(32, V):
+        raise KernelError(f"token_logprobs: {top} alternatives of {V} tokens; at most 32")
+    dev = logits.device
+    out = TokenLogprobs(torch.empty((R,), dtype=torch.float32, device=dev), torch.empty((R,), dtype=torch.float32, device=dev),
+                        torch.empty((R,), dtype=torch.int32, device=dev), torch.empty((R, top), dtype=torch.int32, device=dev),
+                        torch.empty((R, top), dtype=torch.float32, device=dev))
+    if R == 0:
+        return out
+    _on_current(dev, "token_logprobs")
+    _check(_fn("logprobs", "zai_token_logprobs")(
+        out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), out[3].data_ptr(), out[4].data_ptr(), logits.data_ptr(), _dt(logits),
+        logits.stride(0), tokens.data_ptr(), R, V, top, int(blocks), _sm_count(dev), _status_ptr(dev), _stream()), "token_logprobs")
+    return out
+
+
+# ----------------------------------------------------------------------------- steps that check drafted tokens
+MAX_TREE_ROWS = 1024
+
+
+class StepLayout(NamedTuple):
+    """What `step_layout` returns: the step's tables, with a span of no request behind the others for the rows that are left."""
+    cu_q: torch.Tensor                      # [S + 2] int32: first row of each span
+    ctx_lens: torch.Tensor                  # [S + 1] int32
+    positions: torch.Tensor                 # [N] int32
+    seq_idx: torch.Tensor                   # [N] int32
+    kv_slots: torch.Tensor                  # [N] int32: page * page_size + place of the request's i-th new token; -1: none
+    block_tables: torch.Tensor              # [S + 1, width] int32
+    tree_mask: Optional[torch.Tensor]       # [N, words] int32: the rows of its span that a row sees, a bit each (trees only)
+
+
+def _int32(what, *tensors):
+    dev = tensors[0].device
+    for t in tensors:
+        if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous() or t.device != dev:
+            raise KernelError(f"{what}: contiguous int32 tensors on one CUDA device are taken")
+    return dev
+
+
+def _on_current(device, what):
+    if device.index is not None and device.index != torch.cuda.current_device():
+        raise KernelError(f"{what}: the tensors lie on {device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+_sms = {}
+
+
+def _sm_count(device) -> int:
+    n = _sms.get(device.index)
+    if n is None:
+        n = _sms[device.index] = torch.cuda.get_device_properties(device).multi_processor_count
+    return n
+
+
+@_timed("step tables")
+def step_layout(q_lens, ctx_lens, slots, page_rows, page_size, n_rows, width, parents=None, tree_rows=0):
+    """A step's tables from its requests' lengths, all on the device (int32): `q_lens` rows, `ctx_lens` cached positions and the slot of
+    each of S requests; `page_rows` [slots, W], the block table of every slot; `n_rows` rows there is room for; `width` entries
+    of a block table.  `parents` [n_rows]: the rows are trees of drafted tokens of at most `tree_rows` rows each, and a row hangs on
+    this row of its own span (-1: on none); a row's position is then its request's length plus its depth, and `tree_mask` holds
+    its ancestors and itself.  Rows behind the last span belong to a span of no request: the null page, slot -1, nothing seen."""
+    dev = _int32("step_layout", q_lens, ctx_lens, slots, page_rows, *(() if parents is None else (parents,)))
+    S, N, width, tree_rows = q_lens.numel(), int(n_rows), int(width), int(tree_rows) if parents is not None else 0
+    if ctx_lens.shape != q_lens.shape or slots.shape != q_lens.shape or q_lens.dim() != 1 or page_rows.dim() != 2:
+        raise KernelError("step_layout: one length, one context and one slot a request, and the slots' block tables as rows")
+    if parents is not None and (parents.shape != (N,) or not 1 <= tree_rows <= MAX_TREE_ROWS):
+        raise KernelError(f"step_layout: a parent for each of the step's rows, and trees of 1 to {MAX_TREE_ROWS} rows")
+    _on_current(dev, "step_layout")
+    words = (tree_rows + 31) // 32
+    sizes = (S + 2, S + 1, N, N, N, (S + 1) * width, N * words)
+    parts = torch.empty((sum(sizes),), dtype=torch.int32, device=dev).split(sizes)
+    p = [t.data_ptr() for t in parts]
+    _check(_fn("drafts", "zai_step_layout")(
+        *p, q_lens.data_ptr(), ctx_lens.data_ptr(), slots.data_ptr(), page_rows.data_ptr(), _ptr(parents), S, N, width, page_rows.shape[1],
+        page_rows.shape[0], int(page_size), tree_rows, words, _status_ptr(dev), _stream()), "step_layout")
+    return StepLayout(*parts[:5], parts[5].view(S + 1, width), parts[6].view(N, words) if words else None)
+
+
+def _row_heads(t, heads, head_dim, N, what):
+    """Rows [N, heads * head_dim] whose values are contiguous; returns the distance between rows."""
+    if t.shape != (N, heads * head_dim) or t.stride(1) != 1:
+        raise KernelError(f"tree_attention: {what} has rows of {heads} heads of {head_dim} contiguous values")
+    return t.stride(0) if N > 1 else heads * head_dim
+
+
+@_timed("attention")
+def tree_attention(q, k, v, step, cache, heads, kv_heads, head_dim, scale, window=None, impl=None, splits=None):
+    """Attention of drafted rows: row i of a request sees the request's `step.ctx_lens` cached positions in the pages and those
+    rows of its own span whose bit stands in `step.tree_mask` [N, words] (int32; as `step_layout` makes it); keys and values of
+    the step's rows are k and v [N, kv_heads * head_dim] (columns of the projection's rows are fine) and enter no page:
+    `commit_drafts` caches those that are accepted.  `window`: of all these, the ones whose position is above the row's minus the
+    window (`step.positions`: ctx plus the row's depth).  A row that sees nothing gets zeros.  `impl`: "general" or "mma"; `splits`: how
+    many blocks share a tile's keys (None: by the sizes)."""
+    N, H, G, D = q.shape[0], int(heads), int(kv_heads), int(head_dim)
+    if G < 1 or H % G:
+        raise KernelError(f"tree_attention: {H} query heads cannot share {G} key/value heads evenly")
+    pages, bt, mask = cache.pages, cache.block_table, step.tree_mask
+    qs, ks, vs = _row_heads(q, H, D, N, "q"), _row_heads(k, G, D, N, "k"), _row_heads(v, G, D, N, "v")
+    if mask is None:
+        raise KernelError("tree_attention: the step's rows are no trees (no tree_mask)")
+    dev = _int32("tree_attention", mask, bt, step.cu_q, step.ctx_lens, step.positions)
+    S = step.n_seqs
+    if (k.dtype != q.dtype or v.dtype != q.dtype or pages.dtype != q.dtype or q.device != dev or k.device != dev or v.device != dev or pages.device != dev
+            or not pages.is_contiguous() or tuple(pages.shape[1:]) != (2, G, cache.page_size, D) or N != step.n_tokens or mask.shape[0] != N
+            or mask.dim() != 2 or step.positions.numel() != N or step.cu_q.numel() != S + 1 or step.ctx_lens.numel() != S or bt.shape[0] != S):
+        raise KernelError("tree_attention: operands do not fit together")
+    if not (scale > 0.0 and math.isfinite(scale)) or (window is not None and int(window) < 1):
+        raise KernelError("tree_attention: the scale is a positive number, a window at least one position")
+    out = torch.empty((N, H * D), dtype=q.dtype, device=dev)
+    if N == 0 or S == 0:
+        return out
+    _on_current(dev, "tree_attention")
+    group, most = H // G, max(int(step.max_q_len), 1)
+    qp, kp, vp, pp = q.data_ptr(), k.data_ptr(), v.data_ptr(), pages.data_ptr()
+    mma = (q.dtype == torch.bfloat16 and impl != "general" and bool(_fn("tree_attention", "zai_tree_attention_mma_supports")(D))
+           and not ((kp | vp | pp) & 15 or (ks | vs) & 7 or qp & 3 or qs & 1))
+    if impl == "mma" and not mma:
+        raise KernelError("tree_attention: the tensor-core kernel takes bfloat16 heads of 32, 64, 96 or 128 on 16-byte boundaries")
+    if mma:
+        pairs = 16
+        while pairs < 128 and pairs < most * group:
+            pairs *= 2
+    else:
+        pairs = _fn("tree_attention", "zai_tree_attention_general_pairs")()
+    tiles = N * group // pairs + S
+    keys = bt.shape[1] * cache.page_size if window is None else min(bt.shape[1] * cache.page_size, int(window))
+    if splits is None:
+        # enough blocks to fill the SMs, and shares of about a thousand keys; no more blocks than tiles of keys
+        splits, want = 1, 3 * _sm_count(dev)
+        while splits < 16 and splits * 128 < keys and (tiles * G * splits * 2 <= want or splits * 1024 < keys):
+            splits *= 2
+    args = (S, N) + ((pairs,) if mma else ()) + (tiles, int(splits), cache.page_size, pages.shape[0], H, G, D, float(scale), int(window or 0),
+                                                 _status_ptr(dev), _stream())
+    _check(_fn("tree_attention", "zai_tree_attention_mma" if mma else "zai_tree_attention_general")(
+        out.data_ptr(), qp, qs, kp, ks, vp, vs, pp, *(() if mma else (_dt(q),)), bt.data_ptr(), bt.shape[1], step.cu_q.data_ptr(),
+        step.ctx_lens.data_ptr(), step.positions.data_ptr(), mask.data_ptr(), mask.shape[1], *args), "tree_attention")
+    return out
+
+
+class AcceptedDrafts(NamedTuple):
+    """What `accept_drafts` returns."""
+    counts: torch.Tensor                    # [S] int32: accepted rows (the span's first row counts)
+    path: torch.Tensor                      # [S, most] int32: the accepted rows of the step, in order; -1 behind them
+    tokens: torch.Tensor                    # [S, most] int32: the tokens chosen at them (the request's new tokens); -1 behind them
+    ctx_lens: torch.Tensor                  # [S] int32: the requests' lengths with them
+
+
+@_timed("sampling")
+def accept_drafts(choices, tokens, parents, step, most):
+    """Which drafted rows stand: from a span's first row on, the first row that hangs on the current one and whose token (`tokens`
+    [N] int32) is the one chosen there (`choices` [N] int32, from `argmax` or `sample` on the rows' logits) is accepted and becomes
+    the current one.  `parents` as in `step_layout`; a span has at most `most` rows.  S accepted paths, the tokens chosen along
+    them, and the requests' lengths with the accepted rows."""
+    dev = _int32("accept_drafts", choices, tokens, parents, step.cu_q, step.ctx_lens)
+    N, S, most = choices.numel(), step.cu_q.numel() - 1, int(most)
+    if tokens.shape != choices.shape or parents.shape != choices.shape or choices.dim() != 1 or step.ctx_lens.numel() != S:
+        raise KernelError("accept_drafts: a choice, a token and a parent a row, a length a span")
+    if not 1 <= most <= MAX_TREE_ROWS:
+        raise KernelError(f"accept_drafts: trees have 1 to {MAX_TREE_ROWS} rows")
+    _on_current(dev, "accept_drafts")
+    counts, path, chosen, ctx = torch.empty((2 * S * (most + 1),), dtype=torch.int32, device=dev).split((S, S * most, S * most, S))
+    if S:
+        _check(_fn("drafts", "zai_accept_drafts")(
+            counts.data_ptr(), path.data_ptr(), chosen.data_ptr(), ctx.data_ptr(), choices.data_ptr(), tokens.data_ptr(), parents.data_ptr(),
+            step.cu_q.data_ptr(), step.ctx_lens.data_ptr(), S, N, most, _status_ptr(dev), _stream()), "accept_drafts")
+    return AcceptedDrafts(counts, path.view(S, most), chosen.view(S, most), ctx)
+
+
+@_timed("q/k norm, rotation, page write")
+def commit_drafts(k, v, path, counts, step, pages):
+    """Keys and values of accepted rows into the cache: the i-th row of `path` [S, most] (the first `counts` of a request's) goes to
+    `step.kv_slots[step.cu_q[s] + i]`.  `pages` [pages, 2, kv_heads, page_size, head_dim] with k and v [N, kv_heads * head_dim], or
+    the planes of several layers [L, pages, ...] with [L, N, ...]; rows may lie apart (columns of a projection)."""
+    dev = _int32("commit_drafts", path, counts, step.cu_q, step.kv_slots)
+    if pages.dim() not in (5, 6) or k.dim() != pages.dim() - 3:
+        raise KernelError("commit_drafts: pages of one layer with rows, or planes of several layers with as many sets of rows")
+    planes = pages.shape[0] if pages.dim() == 6 else 1
+    num_pages, two, G, page_size, D = pages.shape[-5:]
+    N = k.shape[-2]
+    want = ((planes,) if pages.dim() == 6 else ()) + (N, G * D)
+    S = counts.numel()
+    if (two != 2 or tuple(k.shape) != want or tuple(v.shape) != want or k.dtype != pages.dtype or v.dtype != pages.dtype
+            or not pages.is_contiguous() or k.stride(-1) != 1 or v.stride(-1) != 1 or path.dim() != 2 or path.shape[0] != S
+            or step.cu_q.numel() < S + 1 or step.kv_slots.numel() != N or any(t.device != dev for t in (k, v, pages))):
+        raise KernelError("commit_drafts: operands do not fit together")
+    _on_current(dev, "commit_drafts")
+    if S == 0 or N == 0 or planes == 0 or path.shape[1] == 0:
+        return
+    k_plane, v_plane = (k.stride(0), v.stride(0)) if pages.dim() == 6 else (0, 0)
+    _check(_fn("drafts", "zai_commit_drafts")(
+        pages.data_ptr(), k.data_ptr(), v.data_ptr(), k_plane, v_plane, k.stride(-2), v.stride(-2), path.data_ptr(), counts.data_ptr(),
+        step.cu_q.data_ptr(), step.kv_slots.data_ptr(), _dt(k), S, N, path.shape[1], planes, G, D, page_size, num_pages, _status_ptr(dev),
+        _stream()), "commit_drafts")
 
 
 # ----------------------------------------------------------------------------- recurrent mixers and what goes with them
