@@ -128,6 +128,20 @@ def test_tree_attention(dtype, q_lens, ctx, H, G, D, ps, window):
     assert ops().read_status() == 0
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("q_lens,ctx,group", [([1], [0], 1), ([1], [128], 2), ([5], [127], 4), ([64, 3], [1000, 129], 4), ([33, 0, 16, 7], [5000, 3, 0, 640], 4),
+                                              ([128, 40], [300, 2500], 4), ([1] * 40, [7 * i for i in range(40)], 1), ([24, 9] * 17, [900, 0] * 17, 8),
+                                              ([60], [20000], 4), ([2, 2], [70000, 1], 2)])
+@pytest.mark.parametrize("shape", ["mixed", "forest"])
+def test_tree_attention_in_shares(D, q_lens, ctx, group, shape):
+    """The tcgen05 kernel: shares that begin and end inside a unit, units of one and two turns, requests without rows or without a cache."""
+    H, G = 2 * group, 2
+    q, k, v, step, cache, _ = make_tree_step(list(q_lens), list(ctx), H, G, D, 64, BF16, 13, shape, extra_words=1, packed=shape == "mixed")
+    got = ops().tree_attention(q, k, v, step, cache, H, G, D, D ** -0.5, impl="tcgen05")
+    close(got, q, k, v, step, cache, H, G, D, D ** -0.5, None)
+    assert ops().read_status() == 0
+
+
 @pytest.mark.parametrize("dtype,impl", [(F32, None), (BF16, "general"), (BF16, "mma")])
 @pytest.mark.parametrize("splits", [1, 2, 4, 8, 16])
 @pytest.mark.parametrize("D,group,n", [(64, 2, 5), (64, 4, 8), (64, 4, 14), (128, 4, 30), (128, 8, 2)])

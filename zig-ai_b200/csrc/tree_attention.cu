@@ -26,7 +26,7 @@ struct TreeArgs {
     long long q_stride, k_stride, v_stride;                    // in elements
     const int *table, *cu, *ctx, *positions;
     const unsigned* mask;
-    int table_width, words, S, N, page_size, num_pages, H, G, D, window;
+    int table_width, words, S, N, page_size, page_shift, num_pages, H, G, D, window;     // page_shift: of a page size that is a power of two, else -1
     float scale;
     int* status;
 };
@@ -79,22 +79,28 @@ __device__ __forceinline__ bool sees_node(const TreeArgs& a, const Tile& t, int 
     return a.window <= 0 || a.positions[t.first + other] > pos - a.window;
 }
 
+// The page that position `key` lies in.
+__device__ __forceinline__ int page_index(const TreeArgs& a, int key) { return a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size; }
+
 // ---------------------------------------------------------------------------------------------------- the general kernel
 // A block owns 16 pairs, a warp four of them; per tile of 32 keys a lane computes its key's scores with the warp's pairs, the weights go
-// through shared memory, and the lanes share out the columns.  Keys and values are converted to 32 bits on their way to shared memory.
+// through shared memory, and the lanes share out the columns.  Keys and values are 32-bit numbers in shared memory.  What are 32-bit numbers
+// in memory too, with rows on 16-byte boundaries, comes by cp.async up to two tiles ahead (ASYNC); the rest is converted on its way, eight
+// loads in flight a thread.  A key's place is looked up by one thread, a tile before its copies are issued.  What bounds it at a few
+// hundred keys: the chain of a tile (copies' arrival, scores, maximum, sums), so the keys are split over many blocks.
 #define GEN_PAIRS 16
 #define GEN_KEYS 32
 #define GEN_THREADS 128
 
 // The sum p * v of a tile's keys; GUARD: a key that has no weight stays out whatever its value is.
 template <int COLS, bool GUARD>
-__device__ __forceinline__ void add_values(float (&o)[4][COLS], const float* p, const float* v, int D, int lane) {
+__device__ __forceinline__ void add_values(float (&o)[4][COLS], const float* p, const float* v, int D, int D4, int lane) {
     for (int j = 0; j < GEN_KEYS; ++j) {
         const float4 w = *reinterpret_cast<const float4*>(p + 4 * j);
 #pragma unroll
         for (int c = 0; c < COLS; ++c) {
             const int d = lane + 32 * c;
-            const float x = d < D ? v[j * D + d] : 0.f;
+            const float x = d < D ? v[j * D4 + d] : 0.f;
             if (!GUARD || w.x != 0.f) o[0][c] = fmaf(w.x, x, o[0][c]);
             if (!GUARD || w.y != 0.f) o[1][c] = fmaf(w.y, x, o[1][c]);
             if (!GUARD || w.z != 0.f) o[2][c] = fmaf(w.z, x, o[2][c]);
@@ -103,25 +109,97 @@ __device__ __forceinline__ void add_values(float (&o)[4][COLS], const float* p, 
     }
 }
 
-template <typename T, int COLS>
-__global__ void __launch_bounds__(GEN_THREADS) tree_attention_general_kernel(const TreeArgs a, int splits) {
-    extern __shared__ float sm[];
+template <typename T, int COLS, bool ASYNC>
+__global__ void __launch_bounds__(GEN_THREADS) tree_attention_general_kernel(const TreeArgs a, int splits, int stages) {
+    extern __shared__ __align__(16) float sm[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = a.D, group = a.H / a.G, head = blockIdx.y, rank = blockIdx.x % splits;
     const int D4 = (D + 3) & ~3, KS = D4 + 4;                  // a key's row: four floats further than its length, so that lanes meet no bank twice
+    const int stage = GEN_KEYS * (KS + D4);                    // a tile: keys [32][KS], values [32][D4]
     float* qs = sm;                                            // [16][D4]
-    float* ks = qs + GEN_PAIRS * D4;                           // [32][KS]
-    float* vs = ks + GEN_KEYS * KS;                            // [32][D]
-    float* ps = vs + GEN_KEYS * D4;                            // [4 warps][32 keys][4 pairs]
+    float* ring = qs + GEN_PAIRS * D4;                         // [stages][stage]
+    float* ps = ring + stages * stage;                         // [4 warps][32 keys][4 pairs]
     float* ml = ps + GEN_PAIRS * GEN_KEYS;                     // [16][2]
+    const T** where = reinterpret_cast<const T**>(ml + 2 * GEN_PAIRS);     // [2][32][key, value]
     pdl_trigger();
     pdl_wait();
     const Tile t = find_tile(a, blockIdx.x / splits, GEN_PAIRS);
     if (t.s < 0) return;                                       // (the whole cluster's)
     const int pairs = min(t.n * group - t.pair0, GEN_PAIRS);
+    const int first_key = a.window > 0 ? max(t.ctx - a.window + 1, 0) : 0;
+    const int tile0 = first_key / GEN_KEYS, cached = max((t.ctx + GEN_KEYS - 1) / GEN_KEYS - tile0, 0), total = cached + (t.n + GEN_KEYS - 1) / GEN_KEYS;
+    const int from = (int)((long long)total * rank / splits), upto = (int)((long long)total * (rank + 1) / splits);
+    const ZaiTableRow table = {a.table + (size_t)t.s * a.table_width, a.table_width, a.num_pages, a.status};
+
+    auto look_up = [&](int it) {                               // where tile `it`'s keys lie, by the last warp
+        if (warp != GEN_THREADS / 32 - 1 || it >= upto) return;
+        const T *kp = nullptr, *vp = nullptr;
+        if (it >= cached) {
+            const int key = (it - cached) * GEN_KEYS + lane;
+            if (key < t.n) {
+                kp = (const T*)a.k + (long long)(t.first + key) * a.k_stride + head * D;
+                vp = (const T*)a.v + (long long)(t.first + key) * a.v_stride + head * D;
+            }
+        } else {
+            const int key = (tile0 + it) * GEN_KEYS + lane;
+            if (key < t.ctx && key >= first_key) {
+                const int idx = page_index(a, key);
+                kp = (const T*)a.pages + (((long long)table.page(idx) * 2 * a.G + head) * a.page_size + (key - idx * a.page_size)) * D;
+                vp = kp + (long long)a.G * a.page_size * D;
+            }
+        }
+        const T** w = where + ((it & 1) * GEN_KEYS + lane) * 2;
+        w[0] = kp;
+        w[1] = vp;
+    };
+    // tile `it` into its stage; keys that are not there become zeros.  Returns whether a value is not finite (ASYNC: not known here).
+    auto bring = [&](int it) {
+        bool odd = false;
+        if (it < upto) {
+            float *ks = ring + (it % stages) * stage, *vs = ks + GEN_KEYS * KS;
+            const T* const* w = where + (it & 1) * GEN_KEYS * 2;
+            if (ASYNC) {
+                const int quads = D >> 2;
+                for (int e = threadIdx.x; e < GEN_KEYS * quads; e += GEN_THREADS) {
+                    const int j = e / quads, c = (e - j * quads) * 4;
+                    const T *kp = w[2 * j], *vp = w[2 * j + 1];
+                    cp_async16(ks + j * KS + c, kp ? (const void*)(kp + c) : a.pages, kp != nullptr);
+                    cp_async16(vs + j * D4 + c, vp ? (const void*)(vp + c) : a.pages, vp != nullptr);
+                }
+            } else {
+                for (int e0 = threadIdx.x; e0 < GEN_KEYS * D; e0 += 4 * GEN_THREADS) {
+                    float kx[4], vx[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int e = e0 + u * GEN_THREADS, j = e / D, c = e - j * D;
+                        kx[u] = vx[u] = 0.f;
+                        if (e < GEN_KEYS * D && w[2 * j]) {
+                            kx[u] = to_float(w[2 * j][c]);
+                            vx[u] = to_float(w[2 * j + 1][c]);
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int e = e0 + u * GEN_THREADS, j = e / D, c = e - j * D;
+                        if (e >= GEN_KEYS * D) break;
+                        ks[j * KS + c] = kx[u];
+                        vs[j * D4 + c] = vx[u];
+                        odd |= !(fabsf(vx[u]) < INFINITY);
+                    }
+                }
+            }
+        }
+        if (ASYNC) cp_async_commit();
+        return odd;
+    };
     for (int e = threadIdx.x; e < GEN_PAIRS * D4; e += GEN_THREADS) {
         const int r = e / D4, d = e - r * D4, p = t.pair0 + r;
         qs[e] = r < pairs && d < D ? to_float(((const T*)a.q)[(long long)(t.first + p / group) * a.q_stride + (head * group + p % group) * D + d]) : 0.f;
     }
+    if (D4 != D)                                               // the columns behind a key's own: zeros in every stage (never ASYNC)
+        for (int e = threadIdx.x; e < stages * GEN_KEYS * (D4 - D); e += GEN_THREADS) {
+            const int j = e / (D4 - D), c = D + e - j * (D4 - D);
+            ring[(j / GEN_KEYS) * stage + (j % GEN_KEYS) * KS + c] = 0.f;
+        }
     int node[4], pos[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -129,10 +207,6 @@ __global__ void __launch_bounds__(GEN_THREADS) tree_attention_general_kernel(con
         node[i] = r < pairs ? (t.pair0 + r) / group : -1;
         pos[i] = node[i] >= 0 && a.window > 0 ? a.positions[t.first + node[i]] : 0;
     }
-    const int first_key = a.window > 0 ? max(t.ctx - a.window + 1, 0) : 0;
-    const int tile0 = first_key / GEN_KEYS, cached = max((t.ctx + GEN_KEYS - 1) / GEN_KEYS - tile0, 0), total = cached + (t.n + GEN_KEYS - 1) / GEN_KEYS;
-    const int from = (int)((long long)total * rank / splits), upto = (int)((long long)total * (rank + 1) / splits);
-    const ZaiTableRow table = {a.table + (size_t)t.s * a.table_width, a.table_width, a.num_pages, a.status};
     float o[4][COLS], m[4], l[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -141,37 +215,37 @@ __global__ void __launch_bounds__(GEN_THREADS) tree_attention_general_kernel(con
 #pragma unroll
         for (int c = 0; c < COLS; ++c) o[i][c] = 0.f;
     }
+    const int ahead = ASYNC ? stages - 1 : 0;                  // tiles whose copies are on their way
+    for (int it = from; it < from + ahead; ++it) {
+        look_up(it);
+        __syncthreads();
+        bring(it);
+    }
+    look_up(from + ahead);
     for (int it = from; it < upto; ++it) {
         const bool nodes = it >= cached;
         const int key0 = nodes ? (it - cached) * GEN_KEYS : (tile0 + it) * GEN_KEYS;
-        __syncthreads();                                       // (the tile before has been used)
+        const float *ks = ring + (it % stages) * stage, *vs = ks + GEN_KEYS * KS;
         bool odd = false;
-        for (int j = warp; j < GEN_KEYS; j += GEN_THREADS / 32) {
-            const T *kp = nullptr, *vp = nullptr;
-            const int key = key0 + j;
-            if (nodes) {
-                if (key < t.n) {
-                    kp = (const T*)a.k + (long long)(t.first + key) * a.k_stride + head * D;
-                    vp = (const T*)a.v + (long long)(t.first + key) * a.v_stride + head * D;
-                }
-            } else if (key < t.ctx && key >= first_key) {
-                const int idx = key / a.page_size;
-                kp = (const T*)a.pages + (((long long)table.page(idx) * 2 * a.G + head) * a.page_size + (key - idx * a.page_size)) * D;
-                vp = kp + (long long)a.G * a.page_size * D;
+        if (ASYNC) {
+            if (stages == 3) cp_async_wait<1>();
+            else cp_async_wait<0>();                           // (two stages: the only tile on its way)
+            __syncthreads();                                   // (arrived, and the tile before has been used)
+            bring(it + ahead);
+            look_up(it + ahead + 1);
+            if (nodes || a.window > 0) {                       // tiles that some pair sees in part
+                for (int e = lane; e < GEN_KEYS * D4; e += 32) odd |= !(fabsf(vs[e]) < INFINITY);
+                odd = __any_sync(0xffffffffu, odd);
             }
-            for (int d = lane; d < D4; d += 32) {
-                ks[j * KS + d] = kp && d < D ? to_float(kp[d]) : 0.f;
-                if (d < D) {
-                    const float x = vp ? to_float(vp[d]) : 0.f;
-                    odd |= !(fabsf(x) < INFINITY);
-                    vs[j * D + d] = x;
-                }
-            }
+        } else {
+            __syncthreads();                                   // (looked up, and the tile before has been used)
+            odd = bring(it);
+            odd = __syncthreads_or(odd);
+            look_up(it + 1);
         }
-        odd = __syncthreads_or(odd);
         // scores: this lane's key with the warp's pairs
         float s[4] = {0.f, 0.f, 0.f, 0.f};
-        const float* kr = ks + lane * KS;
+        const float* kr = ks + lane * KS;   // (its columns behind D are zeros)
         const float* qr = qs + warp * 4 * D4;
         for (int d = 0; d < D4; d += 4) {
             const float4 k4 = *reinterpret_cast<const float4*>(kr + d);
@@ -202,13 +276,14 @@ __global__ void __launch_bounds__(GEN_THREADS) tree_attention_general_kernel(con
         __syncwarp();
         *reinterpret_cast<float4*>(mine + 4 * lane) = w;
         __syncwarp();
-        if (odd) add_values<COLS, true>(o, mine, vs, D, lane);
-        else add_values<COLS, false>(o, mine, vs, D, lane);
+        if (odd) add_values<COLS, true>(o, mine, vs, D, D4, lane);
+        else add_values<COLS, false>(o, mine, vs, D, D4, lane);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) l[i] = warp_sum(l[i]);
     T* out = (T*)a.out;
     if (splits == 1) {
+        if (ASYNC) cp_async_wait<0>();
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (node[i] < 0) continue;
@@ -221,8 +296,9 @@ __global__ void __launch_bounds__(GEN_THREADS) tree_attention_general_kernel(con
         return;
     }
     // the blocks' parts: O in shared memory (over the tiles), references and sums behind it; every block joins some of the pairs
+    if (ASYNC) cp_async_wait<0>();
     __syncthreads();
-    float* po = ks;                                            // [16][D]
+    float* po = ring;                                            // [16][D]
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int r = warp * 4 + i;
@@ -264,23 +340,23 @@ __global__ void __launch_bounds__(GEN_THREADS) tree_attention_general_kernel(con
 }
 
 // ---------------------------------------------------------------------------------------------------- bfloat16 on mma.sync
-// A block owns 16 WM pairs; its warps are WM rows of 16 pairs times WN shares of every tile of 64 keys, each share with a maximum,
+// A block owns 16 WM pairs; its warps are WM rows of 16 pairs times WN shares of every tile of KEYS keys, each share with a maximum,
 // a sum and an O of its own (joined with those of the cluster's other blocks at the end).  Keys and values come by cp.async, STAGES tiles
 // in a ring; where a tile's 64 keys lie is looked up a turn before its copies are issued, by one thread a key.  Q stays in registers,
 // scores go from the accumulators into the second product's operand without leaving them.  Weights are rounded to bfloat16 there, as
 // the values are; their sum is taken before the rounding, in 32 bits.
-#define KEYS 64
 
-template <int D, int WM, int WN, int STAGES> struct MmaShape {
+template <int D, int WM, int WN, int KEYS, int STAGES> struct MmaShape {
+    static_assert(KEYS <= 32 * WM * WN && KEYS / WN % 16 == 0, "a thread a key looks up where it lies");
     static constexpr int THREADS = 32 * WM * WN, PAIRS = 16 * WM, ROW = D + 8, STAGE = 2 * KEYS * ROW, KW = KEYS / WN, O_ROW = D + 8;
     static constexpr size_t RING = sizeof(bf16) * STAGES * STAGE;
     static constexpr size_t JOIN = sizeof(float) * WN * PAIRS * O_ROW;
     static constexpr size_t SMEM = (RING > JOIN ? RING : JOIN) + sizeof(void*) * 4 * KEYS + sizeof(float) * 2 * WN * PAIRS;
 };
 
-template <int D, int WM, int WN, int STAGES>
+template <int D, int WM, int WN, int KEYS, int STAGES>
 __global__ void __launch_bounds__(32 * WM * WN) tree_attention_mma_kernel(const TreeArgs a, int splits) {
-    using Shape = MmaShape<D, WM, WN, STAGES>;
+    using Shape = MmaShape<D, WM, WN, KEYS, STAGES>;
     constexpr int THREADS = Shape::THREADS, PAIRS = Shape::PAIRS, ROW = Shape::ROW, KW = Shape::KW, NT = KW / 8, O_ROW = Shape::O_ROW;
     constexpr int CHUNKS = D / 8;                              // pieces of 16 bytes a key
     extern __shared__ __align__(16) char smem[];
@@ -300,8 +376,8 @@ __global__ void __launch_bounds__(32 * WM * WN) tree_attention_mma_kernel(const 
     const ZaiTableRow table = {a.table + (size_t)t.s * a.table_width, a.table_width, a.num_pages, a.status};
 
     auto look_up = [&](int it) {                               // where tile `it`'s keys lie, by the first KEYS threads
-        if ((int)threadIdx.x >= KEYS || it >= upto) return;
-        const int j = threadIdx.x;
+        const int j = threadIdx.x;                             // (there are at least as many threads)
+        if (j >= KEYS || it >= upto) return;
         const bf16 *kp = nullptr, *vp = nullptr;
         if (it >= cached) {
             const int key = (it - cached) * KEYS + j;
@@ -312,7 +388,7 @@ __global__ void __launch_bounds__(32 * WM * WN) tree_attention_mma_kernel(const 
         } else {
             const int key = (tile0 + it) * KEYS + j;
             if (key < t.ctx && key >= first_key) {
-                const int idx = key / a.page_size;
+                const int idx = page_index(a, key);
                 kp = (const bf16*)a.pages + (((long long)table.page(idx) * 2 * a.G + head) * a.page_size + (key - idx * a.page_size)) * D;
                 vp = kp + (long long)a.G * a.page_size * D;
             }
@@ -567,9 +643,13 @@ __global__ void __launch_bounds__(32 * WM * WN) tree_attention_mma_kernel(const 
 }
 
 // ---------------------------------------------------------------------------------------------------- launching
-template <typename... K>
-static int launch_cluster(void (*kernel)(K...), unsigned long long* done, dim3 grid, int threads, size_t smem, int splits, cudaStream_t stream,
-                          const TreeArgs& a) {
+static int page_shift_of(int page_size) {
+    int shift = 0;
+    while ((1 << shift) < page_size) ++shift;
+    return 1 << shift == page_size ? shift : -1;
+}
+template <typename... K, typename... Args>
+static int launch_cluster(void (*kernel)(K...), unsigned long long* done, dim3 grid, int threads, size_t smem, int splits, cudaStream_t stream, Args... args) {
     if (zai_first_on_device(done)) {
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
         cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
@@ -588,15 +668,25 @@ static int launch_cluster(void (*kernel)(K...), unsigned long long* done, dim3 g
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    return (int)cudaLaunchKernelEx(&cfg, kernel, a, splits);
+    return (int)cudaLaunchKernelEx(&cfg, kernel, K(args)...);
 }
 
-template <typename T, int COLS>
+template <typename T, int COLS, bool ASYNC>
 static int launch_general(const TreeArgs& a, int tiles, int splits, cudaStream_t stream) {
     static unsigned long long done = 0;
-    const int D4 = (a.D + 3) & ~3;
-    const size_t smem = sizeof(float) * ((size_t)GEN_PAIRS * D4 + GEN_KEYS * (D4 + 4) + GEN_KEYS * D4 + GEN_PAIRS * GEN_KEYS + 2 * GEN_PAIRS);
-    return launch_cluster(tree_attention_general_kernel<T, COLS>, &done, dim3((unsigned)splits * tiles, a.G), GEN_THREADS, smem, splits, stream, a);
+    const size_t D4 = (a.D + 3) & ~3, stage = sizeof(float) * GEN_KEYS * (2 * D4 + 4);
+    const size_t rest = sizeof(float) * (GEN_PAIRS * D4 + GEN_PAIRS * GEN_KEYS + 2 * GEN_PAIRS) + sizeof(void*) * 4 * GEN_KEYS;
+    const int stages = !ASYNC ? 1 : 3 * stage + rest <= 76 * 1024 ? 3 : 2;      // (three of heads of up to 64, or two of 128: two blocks an SM and more)
+    if (stages * stage + rest > 227 * 1024) return ZAI_BAD_SIZE;
+    return launch_cluster(tree_attention_general_kernel<T, COLS, ASYNC>, &done, dim3((unsigned)splits * tiles, a.G), GEN_THREADS, stages * stage + rest,
+                          splits, stream, a, splits, stages);
+}
+template <typename T, bool ASYNC> static int launch_general_cols(const TreeArgs& a, int tiles, int splits, cudaStream_t stream) {
+    if (a.D <= 32) return launch_general<T, 1, ASYNC>(a, tiles, splits, stream);
+    if (a.D <= 64) return launch_general<T, 2, ASYNC>(a, tiles, splits, stream);
+    if (a.D <= 128) return launch_general<T, 4, ASYNC>(a, tiles, splits, stream);
+    if (a.D <= 256) return launch_general<T, 8, ASYNC>(a, tiles, splits, stream);
+    return launch_general<T, 16, false>(a, tiles, splits, stream);
 }
 
 // Pairs of (row, query head) a block of the general kernel owns.
@@ -610,28 +700,26 @@ ZAI_API int zai_tree_attention_general(void* out, const void* q, long long q_str
         D < 1 || D > 512 || words < 1 || table_width < 1 || (long long)N * (H / G) > 0x3fffffff)
         return ZAI_BAD_SIZE;
     const TreeArgs a = {out, q, k, v, pages, q_stride, k_stride, v_stride, table, cu, ctx, positions, (const unsigned*)mask, table_width, words, S, N,
-                        page_size, num_pages, H, G, D, window, scale, status};
-    ZAI_DISPATCH(dtype, {
-        if (D <= 32) return launch_general<T, 1>(a, tiles, splits, stream);
-        if (D <= 64) return launch_general<T, 2>(a, tiles, splits, stream);
-        if (D <= 128) return launch_general<T, 4>(a, tiles, splits, stream);
-        if (D <= 256) return launch_general<T, 8>(a, tiles, splits, stream);
-        return launch_general<T, 16>(a, tiles, splits, stream);
-    });
+                        page_size, page_shift_of(page_size), num_pages, H, G, D, window, scale, status};
+    if (dtype == ZAI_BF16) return launch_general_cols<bf16, false>(a, tiles, splits, stream);
+    if (dtype != ZAI_F32) return ZAI_BAD_DTYPE;
+    const bool wide = !(((uintptr_t)k | (uintptr_t)v | (uintptr_t)pages) & 15) && !((k_stride | v_stride | D) & 3);
+    return wide ? launch_general_cols<float, true>(a, tiles, splits, stream) : launch_general_cols<float, false>(a, tiles, splits, stream);
 }
 
-template <int D, int WM, int WN, int STAGES> static int launch_mma(const TreeArgs& a, int tiles, int splits, cudaStream_t stream) {
-    using Shape = MmaShape<D, WM, WN, STAGES>;
+template <int D, int WM, int WN, int KEYS, int STAGES> static int launch_mma(const TreeArgs& a, int tiles, int splits, cudaStream_t stream) {
+    using Shape = MmaShape<D, WM, WN, KEYS, STAGES>;
     static_assert(Shape::SMEM <= 227 * 1024, "the ring does not fit");
     static unsigned long long done = 0;
-    return launch_cluster(tree_attention_mma_kernel<D, WM, WN, STAGES>, &done, dim3((unsigned)splits * tiles, a.G), Shape::THREADS, Shape::SMEM, splits,
-                          stream, a);
+    return launch_cluster(tree_attention_mma_kernel<D, WM, WN, KEYS, STAGES>, &done, dim3((unsigned)splits * tiles, a.G), Shape::THREADS, Shape::SMEM, splits,
+                          stream, a, splits);
 }
 template <int D> static int launch_mma_pairs(const TreeArgs& a, int pairs, int tiles, int splits, cudaStream_t stream) {
-    if (pairs == 16) return launch_mma<D, 1, 4, 3>(a, tiles, splits, stream);
-    if (pairs == 32) return launch_mma<D, 2, 2, 3>(a, tiles, splits, stream);
-    if (pairs == 64) return launch_mma<D, 4, 1, 3>(a, tiles, splits, stream);
-    if (pairs == 128) return launch_mma<D, 8, 1, 3>(a, tiles, splits, stream);
+    constexpr int KEYS = D <= 64 ? 128 : 64;                   // of a tile where a block has few pairs: 16 KB of keys, two blocks an SM
+    if (pairs == 16) return launch_mma<D, 1, 4, KEYS, 3>(a, tiles, splits, stream);
+    if (pairs == 32) return launch_mma<D, 2, 2, KEYS, 3>(a, tiles, splits, stream);
+    if (pairs == 64) return launch_mma<D, 4, 1, 64, 3>(a, tiles, splits, stream);
+    if (pairs == 128) return launch_mma<D, 8, 1, 64, 3>(a, tiles, splits, stream);
     return ZAI_BAD_SIZE;
 }
 
@@ -649,7 +737,7 @@ ZAI_API int zai_tree_attention_mma(void* out, const void* q, long long q_stride,
     if ((((uintptr_t)k | (uintptr_t)v | (uintptr_t)pages) & 15) || ((k_stride | v_stride) & 7) || ((uintptr_t)q & 3) || (q_stride & 1) || ((uintptr_t)out & 7))
         return ZAI_BAD_SIZE;
     const TreeArgs a = {out, q, k, v, pages, q_stride, k_stride, v_stride, table, cu, ctx, positions, (const unsigned*)mask, table_width, words, S, N,
-                        page_size, num_pages, H, G, D, window, scale, status};
+                        page_size, page_shift_of(page_size), num_pages, H, G, D, window, scale, status};
     switch (D) {
         case 32: return launch_mma_pairs<32>(a, pairs, tiles, splits, stream);
         case 64: return launch_mma_pairs<64>(a, pairs, tiles, splits, stream);

@@ -181,6 +181,12 @@ _SIGNATURES = {
         "zai_tree_attention_mma": [_P, _P, _L, _P, _L, _P, _L, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I,
                                    _F, _I, _P, _P],
     },
+    "tree_attention_tc": {
+        "zai_tree_attention_tc_supports": [_I, _I, _I, _I],
+        "zai_tree_attention_tc_rows": [],
+        "zai_tree_attention_tc_part": [_I],
+        "zai_tree_attention_tc": [_P, _P, _L, _P, _L, _P, _L, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _P, _P],
+    },
     "logprobs": {"zai_token_logprobs": [_P, _P, _P, _P, _P, _P, _I, _L, _P, _I, _I, _I, _I, _I, _P, _P]},
     "sampling": {
         "zai_argmax": [_P, _P, _I, _I, _P, _P],
@@ -1431,18 +1437,34 @@ def tree_attention(q, k, v, step, cache, heads, kv_heads, head_dim, scale, windo
            and not ((kp | vp | pp) & 15 or (ks | vs) & 7 or qp & 3 or qs & 1))
     if impl == "mma" and not mma:
         raise KernelError("tree_attention: the tensor-core kernel takes bfloat16 heads of 32, 64, 96 or 128 on 16-byte boundaries")
+    width = bt.shape[1] * cache.page_size
+    # Trees of more than 32 pairs of a row and a query head over many keys: tcgen05 (us, tcgen05 and mma.sync: 32 trees of 4-24 rows of 32 heads over 8
+    # behind 300-6000 positions 96 and 148, 8 of 16 rows behind 2000 27 and 28; few pairs and few keys: 8 of 8 rows 25 and 20, one of 12
+    # rows behind 1000 positions 19 and 12)
+    tc = (mma and impl != "mma" and window is None and most <= 128 and (impl == "tcgen05" or (most * group > 32 and S * G * width >= 16384))
+          and not (qp & 15 or qs & 7) and bool(_fn("tree_attention_tc", "zai_tree_attention_tc_supports")(D, cache.page_size, pages.shape[0], G)))
+    if impl == "tcgen05" and not tc:
+        raise KernelError("tree_attention: the tcgen05 kernel takes bfloat16 heads of 64 or 128 on 16-byte boundaries, trees of at most 128 rows, no window")
+    if tc:
+        blocks = _sm_count(dev)
+        parts = torch.empty((blocks * _fn("tree_attention_tc", "zai_tree_attention_tc_part")(D),), dtype=torch.float32, device=dev)
+        _check(_fn("tree_attention_tc", "zai_tree_attention_tc")(
+            out.data_ptr(), qp, qs, kp, ks, vp, vs, pp, bt.data_ptr(), bt.shape[1], step.cu_q.data_ptr(), step.ctx_lens.data_ptr(), mask.data_ptr(),
+            mask.shape[1], S, N, blocks, cache.page_size, pages.shape[0], H, G, D, float(scale), parts.data_ptr(), _status_ptr(dev), _stream()),
+            "tree_attention (tcgen05)", 2)
+        return out
     if mma:
         pairs = 16
         while pairs < 128 and pairs < most * group:
             pairs *= 2
     else:
         pairs = _fn("tree_attention", "zai_tree_attention_general_pairs")()
-    tiles = N * group // pairs + S
-    keys = bt.shape[1] * cache.page_size if window is None else min(bt.shape[1] * cache.page_size, int(window))
+    tiles = S if most * group <= pairs else N * group // pairs + S
     if splits is None:
-        # enough blocks to fill the SMs, and shares of about a thousand keys; no more blocks than tiles of keys
-        splits, want = 1, 3 * _sm_count(dev)
-        while splits < 16 and splits * 128 < keys and (tiles * G * splits * 2 <= want or splits * 1024 < keys):
+        # as many blocks to a tile's keys as fill the SMs about twice (us at 1, 4, 8 and 16: 8 trees of 8 rows behind 2000 positions 40, 20, 34, 78; one
+        # behind 30 000 387, 112, 65, 40; 32 of 2 rows 33, 54, 97, 245), and no more than there are pieces of 64 keys
+        splits, keys = 1, width if window is None else min(width, int(window))
+        while splits < 16 and splits * 64 < keys and tiles * G * splits < 256:
             splits *= 2
     args = (S, N) + ((pairs,) if mma else ()) + (tiles, int(splits), cache.page_size, pages.shape[0], H, G, D, float(scale), int(window or 0),
                                                  _status_ptr(dev), _stream())
