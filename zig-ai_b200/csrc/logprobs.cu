@@ -7,18 +7,22 @@
 // A thread keeps m, z, u of what it has seen (rescaled when its maximum grows) and the count for the rank; they are joined at the end.
 //
 // The best tokens.  An entry's key is its value's bits in an order that compares as a whole number, and behind them the complement
-// of its index: keys are all different, and the order of keys is the order wanted.  The first round of the walk (a piece of the row) is split into 32
-// groups by lane; the top-th largest of the groups' largest keys bounds the row's top-th key from below (`top` <= 32), so from then on only keys at or
-// above it are noted in shared memory: some thirty of the first 8192 entries and fewer of each later round, unless the row ascends.  At the end
-// a noted key's rank is the number of noted keys above it.  A row that notes more than there is room for is walked again in steps that
-// cut the list down and raise the bound as they go.
+// of its index: keys are all different, and the order of keys is the order wanted.  The first round of the walk is split into 32 groups by
+// lane; the top-th largest of the groups' largest keys bounds the row's top-th key from below (`top` <= 32), so only keys at or above it are noted in
+// shared memory: some thirty of each 4096 entries.  After 4, 8, 16, .. rounds the list is cut down to the `top` largest, the last of which is the new bound,
+// so that as many rounds again note as many again.  A key's place is the number of noted keys above it.  A row that
+// notes more than there is room for (one that ascends) is walked again in steps that cut the list down as they go.
+//
+// What bounds it: the instructions, six to seven an entry (a load's quarter, half a maximum, half each of the difference, the product with log2 e and the
+// two sums, which take two numbers at a time, the exponential, and two for the rank), so that is what they are kept to: a thread looks for
+// keys to note only where its round's maximum reaches the bound, and 0 times -inf, which only masked tokens bring, is put right afterwards.
 //
 // A row is split over a cluster of up to 16 blocks when there are few rows; the first block joins the parts through distributed shared memory.
 #include <cooperative_groups.h>
 #include "common.cuh"
 namespace cg = cooperative_groups;
 
-#define LP_THREADS 512
+#define LP_THREADS 256
 #define LP_WARPS (LP_THREADS / 32)
 #define LP_ROUND 16                 // entries of a row a thread looks at in one round
 #define LP_ROOM 1024                // noted keys a block has room for
@@ -59,6 +63,35 @@ __device__ __forceinline__ Sums joined(const Sums& a, const Sums& b) {
     return r;
 }
 
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)), "l"(reinterpret_cast<unsigned long long&>(c)));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float pow2_of(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 struct Part { Sums sums; int before, noted; u64 bound; };      // what a block of a row's cluster hands to the first one
 
 // Entries j0 .. j0 + VEC of a row, of which those in [lo, hi) count; others come back as -inf.
@@ -88,6 +121,17 @@ template <> struct Piece<bf16> {
 template <typename T>
 __device__ __forceinline__ void load_round(const T* __restrict__ row, int at, int lo, int hi, float (&x)[LP_ROUND]) {
     constexpr int VEC = Piece<T>::VEC;
+    if (at >= lo && at + LP_THREADS * LP_ROUND <= hi) {        // (all of it counts: nearly every round)
+        const T* from = row + at + (int)threadIdx.x * VEC;
+#pragma unroll
+        for (int u = 0; u < LP_ROUND / VEC; ++u) {
+            float v[VEC];
+            Piece<T>::load(from, u * LP_THREADS * VEC, v);
+#pragma unroll
+            for (int c = 0; c < VEC; ++c) x[u * VEC + c] = v[c];
+        }
+        return;
+    }
 #pragma unroll
     for (int u = 0; u < LP_ROUND / VEC; ++u) {
         const int j = at + (u * LP_THREADS + (int)threadIdx.x) * VEC;
@@ -118,7 +162,7 @@ __device__ __forceinline__ void select_largest(const u64* list, int n, int keep,
 }
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(float* __restrict__ logprobs, float* __restrict__ entropy,
+__global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_kernel(float* __restrict__ logprobs, float* __restrict__ entropy,
         int* __restrict__ ranks, int* __restrict__ top_ids, float* __restrict__ top_logprobs, const T* __restrict__ logits, long long stride,
         const int* __restrict__ targets, int V, int top, int blocks, int* status) {
     constexpr int VEC = Piece<T>::VEC;
@@ -158,48 +202,26 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(float* __
     int before = 0;
     u64 bound = 0;
     float bound_x = -INFINITY;
-    float x[LP_ROUND], nx[LP_ROUND];
     const int step = LP_THREADS * LP_ROUND;
-    load_round<T>(base, first, lo, hi, x);
-    for (int at = first; at < hi; at += step) {
-        if (at + step < hi) load_round<T>(base, at + step, lo, hi, nx);
-        float top_x = x[0];
+    auto round = [&](const float (&x)[LP_ROUND], int at) {
+        float top4[LP_ROUND / 4], top_x;
 #pragma unroll
-        for (int e = 1; e < LP_ROUND; ++e) top_x = fmaxf(top_x, x[e]);
-        if (TOP) {
-            if (at == first) {                                 // (every block takes part, one without entries too: below)
-                u64 k = 0;
+        for (int e = 0; e < LP_ROUND; e += 4) top4[e / 4] = fmaxf(max3(x[e], x[e + 1], x[e + 2]), x[e + 3]);
+        top_x = fmaxf(max3(top4[0], top4[1], top4[2]), top4[3]);
+        if (TOP && (top_x >= bound_x || top_x != top_x)) {
 #pragma unroll
-                for (int e = 0; e < LP_ROUND; ++e) {
-                    const int j = index_in_round<T>(at, e);
-                    if (j >= lo && j < hi) k = max(k, key_of(x[e], j - lead));
-                }
-                warp_best[t] = k;
-                __syncthreads();
-                if (warp == 0) {
+            for (int e4 = 0; e4 < LP_ROUND; e4 += 4) {
+                if (!(top4[e4 / 4] >= bound_x) && bound_x != -INFINITY) continue;
 #pragma unroll
-                    for (int w = 1; w < LP_WARPS; ++w) k = max(k, warp_best[w * 32 + lane]);
-                    groups[lane] = k;
-                    __syncwarp();
-                    int above = 0;
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) above += groups[i] > k || (groups[i] == k && i < lane);   // (groups without entries are equal)
-                    if (above == top - 1) bound_s = k;
-                }
-                __syncthreads();
-                bound = bound_s;
-                bound_x = fmaxf(value_of(bound), -INFINITY);    // (no bound, or one that is not a number: everything)
-            }
-            if (top_x >= bound_x || top_x != top_x) {
-#pragma unroll
-                for (int e = 0; e < LP_ROUND; ++e) {
-                    const int j = index_in_round<T>(at, e);
-                    const u64 k = key_of(x[e], j - lead);
-                    if (k >= bound && j >= lo && j < hi) {
-                        const int p = atomicAdd(&noted, 1);
-                        if (p < LP_ROOM) list[p] = k;
+                for (int e = e4; e < e4 + 4; ++e)
+                    if (x[e] >= bound_x || x[e] != x[e]) {
+                        const int j = index_in_round<T>(at, e);
+                        const u64 k = key_of(x[e], j - lead);
+                        if (k >= bound && j >= lo && j < hi) {
+                            const int p = atomicAdd(&noted, 1);
+                            if (p < LP_ROOM) list[p] = k;
+                        }
                     }
-                }
             }
         }
         if (top_x > mine.m) {
@@ -207,31 +229,102 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(float* __
             mine = joined(mine, none);
         }
         if (mine.m != -INFINITY) {
+            float2 z = make_float2(0.f, 0.f), u = z;
+            const float2 m2 = make_float2(-mine.m, -mine.m), l2 = make_float2(1.4426950408889634f, 1.4426950408889634f);
 #pragma unroll
-            for (int e = 0; e < LP_ROUND; ++e) {
-                const float d = x[e] - mine.m, w = exp_of(d);
-                mine.z += w;
-                mine.u += w * fmaxf(d, -150.f);                // (of -inf: 0, not 0 times infinity)
+            for (int e = 0; e < LP_ROUND; e += 2) {
+                const float2 d = add2(make_float2(x[e], x[e + 1]), m2), p = mul2(d, l2), w = make_float2(pow2_of(p.x), pow2_of(p.y));
+                z = add2(z, w);
+                u = fma2(w, d, u);
             }
+            if (u.x != u.x || u.y != u.y) {                    // 0 times -inf, which is 0 here
+                u = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int e = 0; e < LP_ROUND; ++e) {
+                    const float d = x[e] - mine.m;
+                    u.x += exp_of(d) * fmaxf(d, -150.f);
+                }
+            }
+            mine.z += z.x + z.y;
+            mine.u += u.x + u.y;
         } else {
 #pragma unroll
             for (int e = 0; e < LP_ROUND; ++e)
                 if (x[e] != x[e]) mine = {0.f, NAN, NAN};      // (nothing else than -inf so far)
         }
+        if (jt < at || jt >= at + step) {                      // (the token is not in this round: one bound for all)
+            const float need = at < jt ? xt : above_xt;
+            int n0 = 0, n1 = 0;
 #pragma unroll
-        for (int u = 0; u < LP_ROUND / VEC; ++u) {
-            const int j = index_in_round<T>(at, u * VEC);
-            if (jt < j || jt >= j + VEC) {
-                const float need = j < jt ? xt : above_xt;
+            for (int e = 0; e < LP_ROUND; e += 2) {
+                n0 += x[e] >= need;
+                n1 += x[e + 1] >= need;
+            }
+            before += n0 + n1;
+        } else {
 #pragma unroll
-                for (int c = 0; c < VEC; ++c) before += x[u * VEC + c] >= need;
-            } else {
+            for (int e = 0; e < LP_ROUND; ++e) before += x[e] >= (index_in_round<T>(at, e) < jt ? xt : above_xt);
+        }
+    };
+    // two rounds at a time, each asked for while the other is looked at
+    float x[LP_ROUND], y[LP_ROUND];
+    load_round<T>(base, first, lo, hi, x);
+    if (first + step < hi) load_round<T>(base, first + step, lo, hi, y);
+    if (TOP && first < hi) {
+        // the first bound: the top-th largest of the groups' largest keys
+        u64 k = 0;
+        float top_x = x[0];
 #pragma unroll
-                for (int c = 0; c < VEC; ++c) before += x[u * VEC + c] >= (j + c < jt ? xt : above_xt);
+        for (int e = 1; e < LP_ROUND; ++e) top_x = fmaxf(top_x, x[e]);
+        if (top_x > -INFINITY) {
+            int e0 = 0;                                        // the first of the largest
+#pragma unroll
+            for (int e = LP_ROUND - 1; e >= 0; --e) e0 = x[e] == top_x ? e : e0;
+            k = key_of(top_x, index_in_round<T>(first, e0) - lead);
+        } else                                                 // nothing but -inf, or what is not a number: which of them are the share's is looked at
+#pragma unroll 1
+            for (int e = 0; e < LP_ROUND; ++e) {
+                const int j = index_in_round<T>(first, e);
+                if (j >= lo && j < hi) k = max(k, key_of(to_float(base[j]), j - lead));
+            }
+        warp_best[t] = k;
+        __syncthreads();
+        if (warp == 0) {
+#pragma unroll
+            for (int w = 1; w < LP_WARPS; ++w) k = max(k, warp_best[w * 32 + lane]);
+            groups[lane] = k;
+            __syncwarp();
+            int above = 0;
+#pragma unroll 8
+            for (int i = 0; i < 32; ++i) above += groups[i] > k || (groups[i] == k && i < lane);   // (groups without entries are equal)
+            if (above == top - 1) bound_s = k;
+        }
+        __syncthreads();
+        bound = bound_s;
+        bound_x = fmaxf(value_of(bound), -INFINITY);           // (no bound, or one that is not a number: everything)
+    }
+    for (int at = first, number = 2; at < hi; at += 2 * step, number += 2) {
+        round(x, at);
+        if (at + 2 * step < hi) load_round<T>(base, at + 2 * step, lo, hi, x);
+        if (at + step < hi) {
+            round(y, at + step);
+            if (at + 3 * step < hi) load_round<T>(base, at + 3 * step, lo, hi, y);
+        }
+        if (TOP && (number & (number - 1)) == 0 && number >= 4 && at + 3 * step < hi) {
+            // after 4, 8, 16, .. rounds: the list cut down to the largest so far, and the bound raised
+            __syncthreads();
+            const int n = noted;
+            __syncthreads();
+            if (n > top && n <= LP_ROOM) {
+                select_largest(list, n, top, best);
+                if (t < top) list[t] = best[t];
+                if (t == 0) noted = top;
+                bound = best[top - 1];
+                bound_x = fmaxf(value_of(bound), -INFINITY);
+                if (t == 0) bound_s = bound;
+                __syncthreads();
             }
         }
-#pragma unroll
-        for (int e = 0; e < LP_ROUND; ++e) x[e] = nx[e];
     }
     if (xt == -INFINITY && asked) {
         // entries outside [lo, hi) came as -inf and were counted as equal ones before the token: counted again, by index
@@ -318,9 +411,9 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(float* __
             }
             if (TOP) {
                 // the other blocks' keys at or above the highest bound, behind this block's own (at most LP_ROOM in all)
-                if (warp > 0 && warp < blocks) {
-                    const int count = cluster.map_shared_rank(&part, warp)->noted;
-                    const u64* theirs = cluster.map_shared_rank(list, warp);
+                for (int other = warp ? warp : LP_WARPS; other < blocks; other += LP_WARPS) {        // (a warp a block, or two)
+                    const int count = cluster.map_shared_rank(&part, other)->noted;
+                    const u64* theirs = cluster.map_shared_rank(list, other);
                     for (int i = lane; i < count; i += 32) {
                         const u64 k = theirs[i];
                         if (k >= low) list[atomicAdd(&noted, 1)] = k;
@@ -380,6 +473,6 @@ ZAI_API int zai_token_logprobs(float* logprobs, float* entropy, int* ranks, int*
         (blocks & (blocks - 1)))
         return ZAI_BAD_SIZE;
     if (blocks == 0)
-        for (blocks = 1; blocks < 16 && (long long)R * blocks * 2 <= 2 * sms && V / (blocks * 2) >= LP_THREADS * LP_ROUND / 2;) blocks *= 2;
+        for (blocks = 1; blocks < 8 && (long long)R * blocks * 2 <= 2 * sms && V / (blocks * 2) >= LP_THREADS * LP_ROUND / 2;) blocks *= 2;
     ZAI_DISPATCH(dtype, return launch_logprobs<T>(logprobs, entropy, ranks, top_ids, top_logprobs, logits, stride, targets, R, V, top, blocks, status, stream));
 }

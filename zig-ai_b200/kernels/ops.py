@@ -341,8 +341,14 @@ def end_forward() -> None:
     _stream_handle = None
 
 
+# The current stream's handle without an object around it (0.2 us a launch instead of 3.3, where torch has the lookup)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream():
-    return _stream_handle if _stream_handle is not None else torch.cuda.current_stream().cuda_stream
+    if _stream_handle is not None:
+        return _stream_handle
+    return torch.cuda.current_stream().cuda_stream if _raw_stream is None else _raw_stream(torch.cuda.current_device())
 
 
 
@@ -1323,9 +1329,8 @@ def token_logprobs(logits, tokens, top=0, blocks=0):
     if not 0 <= top <= min(32, V):
         raise KernelError(f"token_logprobs: {top} alternatives of {V} tokens; at most 32")
     dev = logits.device
-    out = TokenLogprobs(torch.empty((R,), dtype=torch.float32, device=dev), torch.empty((R,), dtype=torch.float32, device=dev),
-                        torch.empty((R,), dtype=torch.int32, device=dev), torch.empty((R, top), dtype=torch.int32, device=dev),
-                        torch.empty((R, top), dtype=torch.float32, device=dev))
+    out = TokenLogprobs(logits.new_empty((R,), dtype=torch.float32), logits.new_empty((R,), dtype=torch.float32), torch.empty_like(tokens),
+                        tokens.new_empty((R, top)), logits.new_empty((R, top), dtype=torch.float32))
     if R == 0:
         return out
     _on_current(dev, "token_logprobs")
@@ -1351,15 +1356,16 @@ class StepLayout(NamedTuple):
 
 
 def _int32(what, *tensors):
-    dev = tensors[0].device
+    """The device of contiguous int32 tensors that lie on one."""
+    index = tensors[0].get_device()
     for t in tensors:
-        if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous() or t.device != dev:
+        if t.dtype is not torch.int32 or t.get_device() != index or index < 0 or not t.is_contiguous():
             raise KernelError(f"{what}: contiguous int32 tensors on one CUDA device are taken")
-    return dev
+    return tensors[0].device
 
 
 def _on_current(device, what):
-    if device.index is not None and device.index != torch.cuda.current_device():
+    if device.index != torch.cuda.current_device():
         raise KernelError(f"{what}: the tensors lie on {device}, the current device is cuda:{torch.cuda.current_device()}")
 
 
@@ -1389,19 +1395,12 @@ def step_layout(q_lens, ctx_lens, slots, page_rows, page_size, n_rows, width, pa
     _on_current(dev, "step_layout")
     words = (tree_rows + 31) // 32
     sizes = (S + 2, S + 1, N, N, N, (S + 1) * width, N * words)
-    parts = torch.empty((sum(sizes),), dtype=torch.int32, device=dev).split(sizes)
+    parts = q_lens.new_empty((sum(sizes),)).split_with_sizes(sizes)
     p = [t.data_ptr() for t in parts]
     _check(_fn("drafts", "zai_step_layout")(
         *p, q_lens.data_ptr(), ctx_lens.data_ptr(), slots.data_ptr(), page_rows.data_ptr(), _ptr(parents), S, N, width, page_rows.shape[1],
         page_rows.shape[0], int(page_size), tree_rows, words, _status_ptr(dev), _stream()), "step_layout")
     return StepLayout(*parts[:5], parts[5].view(S + 1, width), parts[6].view(N, words) if words else None)
-
-
-def _row_heads(t, heads, head_dim, N, what):
-    """Rows [N, heads * head_dim] whose values are contiguous; returns the distance between rows."""
-    if t.shape != (N, heads * head_dim) or t.stride(1) != 1:
-        raise KernelError(f"tree_attention: {what} has rows of {heads} heads of {head_dim} contiguous values")
-    return t.stride(0) if N > 1 else heads * head_dim
 
 
 @_timed("attention")
@@ -1412,22 +1411,28 @@ def tree_attention(q, k, v, step, cache, heads, kv_heads, head_dim, scale, windo
     `commit_drafts` caches those that are accepted.  `window`: of all these, the ones whose position is above the row's minus the
     window (`step.positions`: ctx plus the row's depth).  A row that sees nothing gets zeros.  `impl`: "general" or "mma"; `splits`: how
     many blocks share a tile's keys (None: by the sizes)."""
-    N, H, G, D = q.shape[0], int(heads), int(kv_heads), int(head_dim)
+    N, H, G, D, S = q.shape[0], int(heads), int(kv_heads), int(head_dim), step.n_seqs
     if G < 1 or H % G:
         raise KernelError(f"tree_attention: {H} query heads cannot share {G} key/value heads evenly")
-    pages, bt, mask = cache.pages, cache.block_table, step.tree_mask
-    qs, ks, vs = _row_heads(q, H, D, N, "q"), _row_heads(k, G, D, N, "k"), _row_heads(v, G, D, N, "v")
+    pages, bt, mask, cu_q, ctx_lens, positions = cache.pages, cache.block_table, step.tree_mask, step.cu_q, step.ctx_lens, step.positions
     if mask is None:
         raise KernelError("tree_attention: the step's rows are no trees (no tree_mask)")
-    dev = _int32("tree_attention", mask, bt, step.cu_q, step.ctx_lens, step.positions)
-    S = step.n_seqs
-    if (k.dtype != q.dtype or v.dtype != q.dtype or pages.dtype != q.dtype or q.device != dev or k.device != dev or v.device != dev or pages.device != dev
-            or not pages.is_contiguous() or tuple(pages.shape[1:]) != (2, G, cache.page_size, D) or N != step.n_tokens or mask.shape[0] != N
-            or mask.dim() != 2 or step.positions.numel() != N or step.cu_q.numel() != S + 1 or step.ctx_lens.numel() != S or bt.shape[0] != S):
+    dev = _int32("tree_attention", mask, bt, cu_q, ctx_lens, positions)
+    if q.shape != (N, H * D) or k.shape != (N, G * D) or v.shape != (N, G * D):
+        raise KernelError(f"tree_attention: q, k and v are rows of {H}, {G} and {G} heads of {D}")
+    (qs, q1), (ks, k1), (vs, v1) = q.stride(), k.stride(), v.stride()
+    index, dtype = mask.get_device(), q.dtype
+    if (q1 != 1 or k1 != 1 or v1 != 1 or k.dtype is not dtype or v.dtype is not dtype or pages.dtype is not dtype or q.get_device() != index
+            or k.get_device() != index or v.get_device() != index or pages.get_device() != index or not pages.is_contiguous()
+            or pages.shape[1:] != (2, G, cache.page_size, D) or N != step.n_tokens or mask.dim() != 2 or mask.shape[0] != N
+            or positions.numel() != N or cu_q.numel() != S + 1 or ctx_lens.numel() != S or bt.shape[0] != S):
         raise KernelError("tree_attention: operands do not fit together")
+    if N == 1:                                                 # (the distance between rows means nothing)
+        qs, ks, vs = H * D, G * D, G * D
+    scale = float(scale)
     if not (scale > 0.0 and math.isfinite(scale)) or (window is not None and int(window) < 1):
         raise KernelError("tree_attention: the scale is a positive number, a window at least one position")
-    out = torch.empty((N, H * D), dtype=q.dtype, device=dev)
+    out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((N, H * D))
     if N == 0 or S == 0:
         return out
     _on_current(dev, "tree_attention")
@@ -1447,11 +1452,10 @@ def tree_attention(q, k, v, step, cache, heads, kv_heads, head_dim, scale, windo
         raise KernelError("tree_attention: the tcgen05 kernel takes bfloat16 heads of 64 or 128 on 16-byte boundaries, trees of at most 128 rows, no window")
     if tc:
         blocks = _sm_count(dev)
-        parts = torch.empty((blocks * _fn("tree_attention_tc", "zai_tree_attention_tc_part")(D),), dtype=torch.float32, device=dev)
+        parts = q.new_empty((blocks * _fn("tree_attention_tc", "zai_tree_attention_tc_part")(D),), dtype=torch.float32)
         _check(_fn("tree_attention_tc", "zai_tree_attention_tc")(
-            out.data_ptr(), qp, qs, kp, ks, vp, vs, pp, bt.data_ptr(), bt.shape[1], step.cu_q.data_ptr(), step.ctx_lens.data_ptr(), mask.data_ptr(),
-            mask.shape[1], S, N, blocks, cache.page_size, pages.shape[0], H, G, D, float(scale), parts.data_ptr(), _status_ptr(dev), _stream()),
-            "tree_attention (tcgen05)", 2)
+            out.data_ptr(), qp, qs, kp, ks, vp, vs, pp, bt.data_ptr(), bt.shape[1], cu_q.data_ptr(), ctx_lens.data_ptr(), mask.data_ptr(), mask.shape[1],
+            S, N, blocks, cache.page_size, pages.shape[0], H, G, D, scale, parts.data_ptr(), _status_ptr(dev), _stream()), "tree_attention (tcgen05)", 2)
         return out
     if mma:
         pairs = 16
@@ -1466,11 +1470,15 @@ def tree_attention(q, k, v, step, cache, heads, kv_heads, head_dim, scale, windo
         splits, keys = 1, width if window is None else min(width, int(window))
         while splits < 16 and splits * 64 < keys and tiles * G * splits < 256:
             splits *= 2
-    args = (S, N) + ((pairs,) if mma else ()) + (tiles, int(splits), cache.page_size, pages.shape[0], H, G, D, float(scale), int(window or 0),
-                                                 _status_ptr(dev), _stream())
-    _check(_fn("tree_attention", "zai_tree_attention_mma" if mma else "zai_tree_attention_general")(
-        out.data_ptr(), qp, qs, kp, ks, vp, vs, pp, *(() if mma else (_dt(q),)), bt.data_ptr(), bt.shape[1], step.cu_q.data_ptr(),
-        step.ctx_lens.data_ptr(), step.positions.data_ptr(), mask.data_ptr(), mask.shape[1], *args), "tree_attention")
+    tail = (tiles, int(splits), cache.page_size, pages.shape[0], H, G, D, scale, int(window or 0), _status_ptr(dev), _stream())
+    if mma:
+        _check(_fn("tree_attention", "zai_tree_attention_mma")(
+            out.data_ptr(), qp, qs, kp, ks, vp, vs, pp, bt.data_ptr(), bt.shape[1], cu_q.data_ptr(), ctx_lens.data_ptr(), positions.data_ptr(),
+            mask.data_ptr(), mask.shape[1], S, N, pairs, *tail), "tree_attention")
+    else:
+        _check(_fn("tree_attention", "zai_tree_attention_general")(
+            out.data_ptr(), qp, qs, kp, ks, vp, vs, pp, _dt(q), bt.data_ptr(), bt.shape[1], cu_q.data_ptr(), ctx_lens.data_ptr(), positions.data_ptr(),
+            mask.data_ptr(), mask.shape[1], S, N, *tail), "tree_attention (general)")
     return out
 
 
@@ -1495,12 +1503,13 @@ def accept_drafts(choices, tokens, parents, step, most):
     if not 1 <= most <= MAX_TREE_ROWS:
         raise KernelError(f"accept_drafts: trees have 1 to {MAX_TREE_ROWS} rows")
     _on_current(dev, "accept_drafts")
-    counts, path, chosen, ctx = torch.empty((2 * S * (most + 1),), dtype=torch.int32, device=dev).split((S, S * most, S * most, S))
+    counts, ctx, path = torch.empty_like(step.ctx_lens), torch.empty_like(step.ctx_lens), choices.new_empty((S, most))
+    chosen = torch.empty_like(path)
     if S:
         _check(_fn("drafts", "zai_accept_drafts")(
             counts.data_ptr(), path.data_ptr(), chosen.data_ptr(), ctx.data_ptr(), choices.data_ptr(), tokens.data_ptr(), parents.data_ptr(),
             step.cu_q.data_ptr(), step.ctx_lens.data_ptr(), S, N, most, _status_ptr(dev), _stream()), "accept_drafts")
-    return AcceptedDrafts(counts, path.view(S, most), chosen.view(S, most), ctx)
+    return AcceptedDrafts(counts, path, chosen, ctx)
 
 
 @_timed("q/k norm, rotation, page write")
