@@ -152,14 +152,16 @@ def test_tree_attention_by_every_split(dtype, impl, splits, D, group, n):
     close(got, q, k, v, step, cache, 2 * group, 2, D, D ** -0.5, None)
 
 
-@pytest.mark.parametrize("dtype,impl", [(F32, None), (BF16, "general"), (BF16, "mma")])
-@pytest.mark.parametrize("splits", [1, 4])
+IMPLS = [(F32, None, 1), (F32, None, 4), (BF16, "general", 1), (BF16, "general", 4), (BF16, "mma", 1), (BF16, "mma", 4), (BF16, "tcgen05", None)]
+
+
+@pytest.mark.parametrize("dtype,impl,splits", IMPLS)
 def test_rows_that_see_nothing_and_empty_spans(dtype, impl, splits):
     """A mask without bits over an empty cache gives zeros; spans without rows take no part."""
     q, k, v, step, cache, _ = make_tree_step([4, 6, 3], [0, 50, 0], 4, 2, 64, 16, dtype, 3)
     step.tree_mask[1] = 0
     step.tree_mask[10:13] = 0
-    step.cu_q = ints([0, 4, 4, 10, 13, 13])
+    step.cu_q = ints([0, 4, 4, 10, 13, 13])                    # (a span without rows has a length and a table all the same)
     step.ctx_lens, step.n_seqs = ints([0, 900, 50, 0, 7]), 5
     cache.block_table = cache.block_table[[0, 1, 1, 2, 1]].contiguous()
     got = ops().tree_attention(q, k, v, step, cache, 4, 2, 64, 0.125, impl=impl, splits=splits)
@@ -167,7 +169,7 @@ def test_rows_that_see_nothing_and_empty_spans(dtype, impl, splits):
     assert not got[[1, 10, 11, 12]].any()
 
 
-@pytest.mark.parametrize("dtype,impl", [(F32, None), (BF16, "general"), (BF16, "mma")])
+@pytest.mark.parametrize("dtype,impl", [(F32, None), (BF16, "general"), (BF16, "mma"), (BF16, "tcgen05")])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_what_is_not_finite_reaches_the_rows_that_see_it_alone(dtype, impl, bad):
     H, G, D = 4, 2, 64
@@ -184,6 +186,8 @@ def test_what_is_not_finite_reaches_the_rows_that_see_it_alone(dtype, impl, bad)
     hit = hit.view(79, -1)
     assert torch.equal(got[~hit], want[~hit])
     assert not torch.isfinite(got[hit]).any()
+    if impl == "tcgen05":                                    # (takes no window)
+        return
     # a window's edge inside a tile of cached keys
     q, k, v, step, cache, _ = make_tree_step([6], [90], H, G, D, 16, dtype, 6, "chain")
     clean = ops().tree_attention(q, k, v, step, cache, H, G, D, 0.125, 20, impl=impl, splits=1)
@@ -191,6 +195,36 @@ def test_what_is_not_finite_reaches_the_rows_that_see_it_alone(dtype, impl, bad)
     cache.pages[page, 1, :, off] = bad                       # position 72: rows at 90 and 91 see it (72 > 91 - 20), those behind do not
     got = ops().tree_attention(q, k, v, step, cache, H, G, D, 0.125, 20, impl=impl, splits=1)
     assert torch.equal(got[2:], clean[2:]) and not torch.isfinite(got[:2]).any()
+
+
+@pytest.mark.parametrize("dtype,impl", [(F32, None), (BF16, "general"), (BF16, "mma"), (BF16, "tcgen05")])
+@pytest.mark.parametrize("grow", [0.02, 6.0, 40.0])
+def test_scores_that_grow_along_the_keys(dtype, impl, grow):
+    """The running maximum moves tile by tile, by little or by hundreds; the last keys, or the drafted rows, outweigh all before them."""
+    H, G, D = 8, 2, 64
+    for ctx in (700, 300):
+        q, k, v, step, cache, _ = make_tree_step([9, 40], [ctx, 1100], H, G, D, 16, dtype, 5)
+        q[:, ::64] = 8.0                                    # (every head's first column)
+        for s in range(2):
+            n = int(step.ctx_lens[s])
+            table = cache.block_table[s].tolist()
+            for j in range(0, n, 5):
+                cache.pages[table[j // 16], 0, :, j % 16, 0] = grow * j / 128
+        k[4, ::64] = grow * 9
+        got = ops().tree_attention(q, k, v, step, cache, H, G, D, 0.125, impl=impl)
+        # (scores of hundreds: their rounding is what the bound of `close` is made of, with the largest of all of them)
+        close(got, q, k, v, step, cache, H, G, D, 0.125, None)
+    assert ops().read_status() == 0
+
+
+def test_spans_longer_than_the_step_says_raise_the_status_word():
+    for n, said, impl, dtype in ((9, 2, "mma", BF16), (40, 16, "mma", BF16), (130, 100, "tcgen05", BF16), (30, 3, None, F32)):
+        q, k, v, step, cache, _ = make_tree_step([n, n], [40, 100], 4, 2, 64, 16, dtype, 5)
+        step.max_q_len = n if said == 100 else said
+        if impl == "tcgen05":
+            step.max_q_len = said
+        ops().tree_attention(q, k, v, step, cache, 4, 2, 64, 0.125, impl=impl)
+        assert ops().read_status() == 64, (n, said, impl)
 
 
 def test_tree_attention_large_offsets():
@@ -205,7 +239,7 @@ def test_tree_attention_large_offsets():
     pages[0] = float("nan")
     want = ops().tree_attention(q, k, v, step, cache, H, G, D, 0.125)
     far = SimpleNamespace(pages=pages, page_size=ps, block_table=torch.where(cache.block_table > 0, cache.block_table + n_pages - used, 0).int())
-    for impl in ("mma", "general"):
+    for impl in ("mma", "general", "tcgen05"):
         near = ops().tree_attention(q, k, v, step, cache, H, G, D, 0.125, impl=impl)
         assert torch.equal(ops().tree_attention(q, k, v, step, far, H, G, D, 0.125, impl=impl), near)
     assert want.isfinite().all()
@@ -217,18 +251,19 @@ def test_bad_pages_raise_the_status_word():
     assert ops().read_status() == 0
     bt = cache.block_table.clone()
     bt[0, 3] = cache.pages.shape[0]
-    for impl in ("mma", "general"):
+    for impl in ("mma", "general", "tcgen05"):
         got = ops().tree_attention(q, k, v, step, SimpleNamespace(pages=cache.pages, block_table=bt, page_size=16), 4, 2, 64, 0.125, impl=impl)
         assert ops().read_status() == 4
-        if impl == "mma":
-            assert torch.equal(got[5:], good[5:])
+        assert torch.isfinite(got).all() and (impl != "mma" or torch.equal(got[5:], good[5:]))
     narrow = SimpleNamespace(pages=cache.pages, block_table=cache.block_table[:, :5].contiguous(), page_size=16)
-    ops().tree_attention(q, k, v, step, narrow, 4, 2, 64, 0.125)
-    assert ops().read_status() == 16
+    for impl in ("mma", "general", "tcgen05"):
+        ops().tree_attention(q, k, v, step, narrow, 4, 2, 64, 0.125, impl=impl)
+        assert ops().read_status() == 16
     step.cu_q = ints([0, 5, 99])
     step.n_seqs = 2
-    ops().tree_attention(q, k, v, step, cache, 4, 2, 64, 0.125)
-    assert ops().read_status() == 32
+    for impl in ("mma", "general", "tcgen05"):
+        ops().tree_attention(q, k, v, step, cache, 4, 2, 64, 0.125, impl=impl)
+        assert ops().read_status() == 32
 
 
 def test_unaligned_rows_take_the_general_kernel():
@@ -558,3 +593,83 @@ def test_operators_on_another_stream_and_in_graphs():
         for a, b in zip(out, want):
             assert torch.equal(a, b)
     assert o.read_status() == 0
+
+
+# ------------------------------------------------------------------------------------------------ together, as a model runs them
+@pytest.fixture(scope="module")
+def tree_models(tmp_path_factory):
+    from draft_configs import TREES_A, TREES_B
+    from zig_ai_b200.config import config_from_dict
+    from zig_ai_b200.weights import write_random_model
+    out = {}
+    for name, cfg in (("A", TREES_A), ("B", TREES_B)):
+        out[name] = (str(tmp_path_factory.mktemp("trees") / name), cfg)
+        write_random_model(config_from_dict(cfg), 5, out[name][0], matrix_std="fan_in")
+    return out
+
+
+@pytest.mark.parametrize("name,dtype", [("A", "float32"), ("A", "bfloat16"), ("B", "float32"), ("B", "bfloat16")])
+def test_verified_trees_follow_the_plain_model(tree_models, name, dtype):
+    """Generation by checked drafts: every token is the plain implementation's choice behind the tokens before it (in bfloat16 within what the
+    model's rounding moves its logits, as for single tokens), most steps take more than one, and the cache's bookkeeping holds."""
+    import plain_lfm2
+    from draft_configs import speculate
+    from zig_ai_b200.engine.runner import load_runner
+    d, cfg = tree_models[name]
+    V = cfg["vocab_size"]
+    c, W = plain_lfm2.read_config(d), plain_lfm2.read_weights(d)
+    g = random.Random(2)
+    prompts = {f"r{i}": [g.randrange(V) for _ in range(n)] for i, n in enumerate([1, 19, 60])}
+    truths = {}
+    for rid, p in prompts.items():
+        toks = list(p)
+        for _ in range(30):
+            toks.append(int(plain_lfm2.forward(c, W, toks)[-1].argmax()))
+        truths[rid] = toks[len(p):]
+    runner = load_runner(d, dtype, max_tokens=512, max_requests=4, page_size=16)
+    got, steps = speculate(runner, prompts, 20, truths, g, V)
+    if dtype == "float32":
+        assert got == {r: t[:20] for r, t in truths.items()} and steps < 20
+    for rid, out in got.items():
+        logits = plain_lfm2.forward(c, W, prompts[rid] + out)
+        for i, tok in enumerate(out):
+            row = logits[len(prompts[rid]) + i - 1]
+            assert float(row.max() - row[tok]) <= (1e-3 if dtype == "float32" else 8e-2 * float(row.abs().max()))
+
+
+def test_layout_serves_the_kernels_that_are_there(tree_models):
+    """A step laid out on the device from lengths runs through page writes and span attention as one packed on the host does."""
+    from zig_ai_b200.cache.manager import CacheView
+    from zig_ai_b200.engine.batch import pack_step
+    o, H, G, D, ps = ops(), 4, 2, 64, 16
+    g = torch.Generator(device="cuda").manual_seed(4)
+    ctx, q_lens = [20, 0, 37], [5, 33, 10]
+    table = [[3, 7, 0, 0], [5, 1, 9, 0], [2, 8, 6, 0]]
+    host = pack_step(o, BF16, torch.device("cuda", 0), [(s, ctx[s], [0] * q_lens[s], [], s + 1) for s in range(3)], {0: table})
+    rows = torch.zeros((5, 6), dtype=torch.int32, device="cuda")
+    rows[[4, 1, 3], :4] = ints(table)
+    lay = o.step_layout(ints(q_lens), ints(ctx), ints([4, 1, 3]), rows, ps, 48, 4)
+    assert torch.equal(lay.positions, host.positions) and torch.equal(lay.seq_idx, host.seq_idx) and torch.equal(lay.cu_q[:4], host.cu_q)
+    assert torch.equal(lay.block_tables[:3], host.block_tables[0]) and torch.equal(lay.ctx_lens[:3], host.ctx_lens)
+    q, k, v = (torch.randn((48, n * D), generator=g, device="cuda").to(BF16) for n in (H, G, G))
+    old = torch.randn((10, 2, G, ps, D), generator=g, device="cuda").to(BF16)
+    outs = []
+    for step, bt in ((host, host.block_tables[0]), (SimpleNamespace(**{**vars(host), "positions": lay.positions, "seq_idx": lay.seq_idx, "cu_q": lay.cu_q[:4],
+                                                                       "ctx_lens": lay.ctx_lens[:3]}), lay.block_tables[:3])):
+        view = CacheView(0, old.clone(), bt.contiguous(), ps)
+        o.kv_write(k, v, step, view, G, D)
+        outs.append((view.pages, o.paged_attention(q, step, view, H, G, D, 0.125)))
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+    # a chain of drafts is a span: committing all of its rows writes the pages that kv_write writes
+    pages, path = old.clone(), torch.full((3, 33), -1, dtype=torch.int32)
+    for s, (a, n) in enumerate(zip([0, 5, 38], q_lens)):
+        path[s, :n] = torch.arange(a, a + n)
+    o.commit_drafts(k, v, path.cuda(), ints(q_lens), lay, pages)
+    assert torch.equal(pages, outs[0][0])
+    # and attention over a chain's masks is span attention
+    chain = o.step_layout(ints(q_lens), ints(ctx), ints([4, 1, 3]), rows, ps, 48, 4, ints([i - 1 for n in q_lens for i in range(n)]), 33)
+    assert torch.equal(chain.positions, lay.positions)
+    step = SimpleNamespace(cu_q=chain.cu_q, ctx_lens=chain.ctx_lens, positions=chain.positions, tree_mask=chain.tree_mask, n_seqs=4, n_tokens=48, max_q_len=33)
+    got = o.tree_attention(q, k, v, step, SimpleNamespace(pages=old, block_table=chain.block_tables, page_size=ps), H, G, D, 0.125)
+    # (two kernels that each round the weights and the result to bfloat16: 2 (2^-8 sum p|v| + 2^-8 |o|), |v| < 6)
+    assert float((got.float() - outs[0][1].float()).abs().max()) <= 4 * 2.0 ** -8 * float(v.float().abs().max())

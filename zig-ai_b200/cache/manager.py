@@ -242,6 +242,14 @@ class CacheManager:
         rc.num_tokens = total_tokens
         rc.capacity = min((len(t) for t in rc.tables.values()), default=1 << 40) * self.page_size
 
+    def settle(self, request_id, total_tokens: int) -> None:
+        """Only positions 0..total_tokens-1 of those reserved hold tokens now (drafted tokens that were not accepted have left
+        none); the pages reserved beyond them stay with the request."""
+        rc = self.requests[request_id]
+        if not 0 <= total_tokens <= rc.num_tokens:
+            raise ValueError(f"{total_tokens} positions of request {request_id!r}, which has {rc.num_tokens} reserved")
+        rc.num_tokens = total_tokens
+
     def release(self, request_id) -> None:
         """Give back everything the request holds."""
         rc = self.requests.pop(request_id)

@@ -35,9 +35,11 @@ struct TreeArgs {
 // the span's n * H / G.
 struct Tile { int s, first, n, ctx, pair0; };
 
-// The tile with this number when every span is cut into tiles of M pairs; all lanes of a warp.  s < 0: there is none.
-__device__ __forceinline__ Tile find_tile(const TreeArgs& a, int number, int M) {
+// The tile with this number when every span is cut into tiles of M pairs; all lanes of a warp.  s < 0: there is none.  `last`: no later number
+// is asked for, so a tile behind this one is a row that nobody computes (a span longer than the launch was told).
+__device__ __forceinline__ Tile find_tile(const TreeArgs& a, int number, int M, bool last) {
     const int lane = threadIdx.x & 31, group = a.H / a.G;
+    Tile t = {-1, 0, 0, 0, 0};
     for (int at = 0; at < a.S; at += 32) {
         const int s = at + lane;
         int first = 0, n = 0;
@@ -58,18 +60,27 @@ __device__ __forceinline__ Tile find_tile(const TreeArgs& a, int number, int M) 
         }
         const unsigned here = __ballot_sync(0xffffffffu, number < upto);
         if (here) {
+            if (t.s >= 0) {                                    // (only the last number gets here: there is a tile behind it)
+                zai_raise(a.status, ZAI_ST_TREE);
+                return t;
+            }
             const int w = __ffs(here) - 1;
-            Tile t;
             t.s = at + w;
             t.first = __shfl_sync(0xffffffffu, first, w);
             t.n = __shfl_sync(0xffffffffu, n, w);
             t.pair0 = (number - __shfl_sync(0xffffffffu, upto - tiles, w)) * M;
             t.ctx = max(a.ctx[t.s], 0);
-            return t;
+            if (!last) return t;
+            if (__shfl_sync(0xffffffffu, upto, 31) > number + 1) {
+                zai_raise(a.status, ZAI_ST_TREE);
+                return t;
+            }
+            number = 0;                                        // the first tile of a later span would be this one
+            continue;
         }
-        number -= __shfl_sync(0xffffffffu, upto, 31);
+        number -= t.s >= 0 ? 0 : __shfl_sync(0xffffffffu, upto, 31);
     }
-    return {-1, 0, 0, 0, 0};
+    return t;
 }
 
 // Does row `node` of the tile's span see row `other`?
@@ -122,7 +133,7 @@ __global__ void __launch_bounds__(GEN_THREADS) tree_attention_general_kernel(con
     const T** where = reinterpret_cast<const T**>(ml + 2 * GEN_PAIRS);     // [2][32][key, value]
     pdl_trigger();
     pdl_wait();
-    const Tile t = find_tile(a, blockIdx.x / splits, GEN_PAIRS);
+    const Tile t = find_tile(a, blockIdx.x / splits, GEN_PAIRS, blockIdx.x / splits == gridDim.x / splits - 1);
     if (t.s < 0) return;                                       // (the whole cluster's)
     const int pairs = min(t.n * group - t.pair0, GEN_PAIRS);
     const int first_key = a.window > 0 ? max(t.ctx - a.window + 1, 0) : 0;
@@ -367,7 +378,7 @@ __global__ void __launch_bounds__(32 * WM * WN) tree_attention_mma_kernel(const 
     const int group = a.H / a.G, g = lane >> 2, q4 = lane & 3;
     pdl_trigger();
     pdl_wait();
-    const Tile t = find_tile(a, blockIdx.x / splits, PAIRS);
+    const Tile t = find_tile(a, blockIdx.x / splits, PAIRS, blockIdx.x / splits == gridDim.x / splits - 1);
     if (t.s < 0) return;                                       // (the whole cluster's)
     const int pairs = min(t.n * group - t.pair0, PAIRS);
     const int first_key = a.window > 0 ? max(t.ctx - a.window + 1, 0) : 0;

@@ -40,6 +40,9 @@ class StepBatch:
     attn_tiles: Optional[int] = None   # blocks of query rows to launch for span attention (default: from q_lens);
     #                                    a captured graph launches an upper bound for its bucket of step shapes
     scratch: Dict = field(default_factory=dict)   # what kernels compute once per step (rotation tables)
+    tree_mask: Optional[torch.Tensor] = None      # [N, words] int32: spans are trees of drafted tokens, and a row sees these rows of its own;
+    #                                               layers cache nothing, their keys and values stay in `drafted` until rows are accepted
+    drafted: List = field(default_factory=list)   # per layer call: (k, v, group, pages)
 
 
 @dataclass
@@ -146,6 +149,35 @@ def batch_views(ops, dtype, dev: torch.Tensor, lay: PackedLayout) -> StepBatch:
         max_kv_len=max((c + n for c, n in zip(lay.ctx, lay.q_lens)), default=0),
         decode_only=all(n == 1 for n in lay.q_lens) and S > 0,
         q_lens=lay.q_lens, request_ids=lay.request_ids, kv_lens=[c + n for c, n in zip(lay.ctx, lay.q_lens)])
+
+
+def lay_out_trees(ops, dtype, device, spans, parents, tables: Dict[int, "np.ndarray"], page_size: int, n_rows: int):
+    """The description of a step whose spans are trees of drafted tokens, laid out on the device from the requests' lengths
+    (`ops.step_layout`, once per group of pages): `spans` as in `pack_host` (every row's logits are wanted), `parents` a list per
+    span, `n_rows` rows in all, of which those behind the spans belong to no request.  Returns the StepBatch, the rows' tokens and
+    parents on the device, and the layouts by group."""
+    S, lens, ctx = len(spans), [len(s[2]) for s in spans], [s[1] for s in spans]
+    n, most = sum(lens), max(lens)
+    parts = [lens, ctx, range(S), [t for s in spans for t in s[2]] + [0] * (n_rows - n), [p for ps in parents for p in ps] + [-1] * (n_rows - n), range(n)]
+    parts = [np.asarray(p, dtype=np.int32) for p in parts]
+    tables = {g: np.asarray(t, dtype=np.int32).reshape(S, -1) for g, t in tables.items()}
+    flat = np.concatenate(parts + [t.reshape(-1) for t in tables.values()])
+    host = torch.empty(flat.size, dtype=torch.int32, pin_memory=device.type == "cuda")
+    host.numpy()[:] = flat
+    dev = host.to(device, non_blocking=True) if device.type == "cuda" else host
+    views, at = [], 0
+    for p in parts + list(tables.values()):
+        views.append(dev[at:at + p.size])
+        at += p.size
+    q_lens, ctx_lens, slots, tokens, up, wanted = views[:6]
+    layouts = {g: ops.step_layout(q_lens, ctx_lens, slots, rows.view(S, -1), page_size, n_rows, t.shape[1], up, most)
+               for (g, t), rows in zip(tables.items(), views[6:])}
+    lay = next(iter(layouts.values()))
+    return StepBatch(
+        ops=ops, dtype=dtype, n_tokens=n_rows, n_seqs=S + 1, n_wanted=n, token_ids=tokens, positions=lay.positions, seq_idx=lay.seq_idx, cu_q=lay.cu_q,
+        ctx_lens=lay.ctx_lens, slot_ids=slots, logit_rows=wanted, block_tables={g: x.block_tables for g, x in layouts.items()},
+        max_q_len=max(most, n_rows - n), max_kv_len=max(c + m for c, m in zip(ctx, lens)), q_lens=lens + [n_rows - n],
+        request_ids=[s[0] for s in spans], kv_lens=[c + m for c, m in zip(ctx, lens)], tree_mask=lay.tree_mask), tokens, up, layouts
 
 
 def pack_step(ops, dtype, device, spans, tables: Dict[int, "np.ndarray"], pin: bool = False) -> StepBatch:

@@ -241,6 +241,33 @@ class Engine:
             raise RuntimeError(f"{len(failed)} request(s) could not be served: out of pages")
         return [done[i].output for i in ids]
 
+    def score(self, prompts: Sequence[Sequence[int]], top: int = 0) -> List[List[dict]]:
+        """How likely the model finds given tokens: for every prompt a list with an entry for each token but the first: its log probability
+        behind the tokens before it (`logprob`), its `rank` among all tokens (0: the likeliest), the `entropy` there in nats, and the
+        `top` (at most 32) likeliest tokens with their log probabilities (`top`, pairs).  Runs beside requests that are being
+        served if slots and pages are free; prompts are cut into portions of `max_batched_tokens`."""
+        out = []
+        for k, prompt in enumerate(prompts):
+            tokens, rid, entries = [int(t) for t in prompt], ("score", self._next_id, k), []
+            if not 0 < len(tokens) <= self.max_model_len:
+                raise ValueError(f"a prompt of {len(tokens)} tokens cannot be scored; the model's length is {self.max_model_len}")
+            self.runner.add_request(rid)
+            try:
+                for a in range(0, len(tokens), self.scheduler.max_batched_tokens):
+                    part = tokens[a:a + self.scheduler.max_batched_tokens]
+                    n = min(len(part), len(tokens) - 1 - a)             # (the last token has none behind it)
+                    logits = self.runner.step([(rid, part, list(range(n)))])
+                    if n == 0:
+                        continue
+                    targets = torch.tensor(tokens[a + 1:a + 1 + n], dtype=torch.int32, device=logits.device)
+                    got = [t.tolist() for t in self.runner.ops.token_logprobs(logits, targets, top)]
+                    entries += [dict(token=t, logprob=lp, rank=r, entropy=e, top=list(zip(ids, lps)))
+                                for t, lp, e, r, ids, lps in zip(tokens[a + 1:], *got)]
+            finally:
+                self.runner.end_request(rid)
+            out.append(entries)
+        return out
+
     def warm_up(self, n_seqs: int = 1) -> None:
         """What only the first steps pay (libraries' first calls, the capture of the decode graph for `n_seqs`
         requests), paid now: a request of two tokens is run to its second new token, and the graph of the bucket is

@@ -19,7 +19,8 @@ import torch
 from ..cache import CacheManager, OutOfPages
 from ..cache.manager import NULL_PAGE, NULL_SLOT
 from ..models import build_model
-from .batch import StepBatch, pack_step
+from ..parts.base import Mixer
+from .batch import StepBatch, lay_out_trees, pack_step
 
 
 class StepError(ValueError):
@@ -197,6 +198,49 @@ class ModelRunner:
         if check:
             self.check_status(self.steps - 1)
         return logits
+
+
+    # ------------------------------------------------------------------ drafted tokens
+    def takes_trees(self) -> bool:
+        """Whether `verify` can run this model: every mixer is attention over its own cache (a recurrent state cannot go down several
+        branches at once)."""
+        return (all(getattr(p, "takes_trees", False) for p in self.model.all_parts() if isinstance(p, Mixer)) and bool(self.cache.paged_groups())
+                and all(c.cache_of is None for c in self.model.spec.order) and not self.model.keeps_embedding)
+
+    def verify(self, entries, choose=None) -> List[List[int]]:
+        """Run trees of drafted tokens and keep what the model itself would have chosen.  entries: (request, tokens, parents): tokens[0]
+        is the request's next token, every other one a draft that hangs on an earlier one of the list (parents[0] is -1).  `choose`:
+        the ids to choose, int32 [rows], from 32-bit logits [rows, vocab] (default: the largest).  Returns each request's new
+        tokens: what was chosen at its first token and along the drafts that this met, the last of which is its next token (and is not
+        in the cache yet).  The tokens come out as single tokens would have one after the other."""
+        ops = self.ops
+        if not self.takes_trees():
+            raise StepError("this model has layers that do not run trees of drafted tokens")
+        for rid, tokens, parents in entries:
+            if len(parents) != len(tokens) or len(tokens) < 1 or parents[0] != -1 or any(not 0 <= parents[i] < i for i in range(1, len(parents))):
+                raise StepError(f"request {rid!r}: a draft hangs on a token before it, the first token on none")
+            if len(tokens) > getattr(ops, "MAX_TREE_ROWS", 1024):
+                raise StepError(f"request {rid!r}: a tree of {len(tokens)} tokens")
+        spans, tables = self._reserve([(rid, tokens, []) for rid, tokens, _ in entries])
+        n = sum(len(t) for _, t, _ in entries)
+        pad = 0 if n <= 16 or self.device.type != "cuda" else -n % (32 if n <= 256 else 64)      # (few distinct row counts: see `pad_rows`)
+        step, tokens, parents, layouts = lay_out_trees(ops, self.dtype, self.device, spans, [p for _, _, p in entries], tables, self.cache.page_size, n + pad)
+        logits = self.model.forward(step, self.cache)
+        choices = torch.zeros_like(tokens)
+        choices[:n] = (choose or ops.argmax)(logits)
+        accepted = ops.accept_drafts(choices, tokens, parents, step, step.max_q_len)
+        for k, v, group, pages in step.drafted:
+            ops.commit_drafts(k, v, accepted.path, accepted.counts, layouts[group], pages)
+        counts, chosen = accepted.counts.tolist(), accepted.tokens.tolist()
+        out = []
+        for (rid, _, _), m, row in zip(entries, counts, chosen):
+            self.processed[rid] += m
+            self.cache.settle(rid, self.processed[rid])
+            out.append(row[:m])
+        self.steps += 1
+        self.tokens_run += n
+        self.check_status(self.steps - 1)
+        return out
 
 
 def pad_rows(spans, tables, page_size: int):

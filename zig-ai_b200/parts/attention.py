@@ -134,6 +134,8 @@ class Attention(Mixer):
             self.kernel_libs = type(self).kernel_libs + ("qkv_prepare",)
         if self.differential is not None:
             self.kernel_libs = type(self).kernel_libs + ("attention_difference",)
+        # steps whose spans are trees of drafted tokens: plain (windowed) scores over the layer's own cache
+        self.takes_trees = not self.prepared and self.differential is None and self.kv_proj
 
     def params(self):
         q_dim, kv_dim = self.heads * self.head_dim, self.kv_heads * self.head_dim
@@ -304,7 +306,26 @@ class Attention(Mixer):
             o = ops.attention_difference(o, self.map_heads, self.value_dim, self.cache_dim, self.lam, 1.0 - self.differential, self.eps)
         return ops.linear(o, self.w_o)
 
+    def _forward_tree(self, x, step, cache, write_cache):
+        """A step of drafted trees: the rows' keys and values go into no page but stay with the step (`step.drafted`) until rows are
+        accepted."""
+        if not (self.takes_trees and write_cache):
+            raise ValueError("this attention layer does not run trees of drafted tokens")
+        ops, H, G, D = step.ops, self.heads, self.kv_heads, self.cache_dim
+        qkv = ops.linear(x, self.w_qkv)
+        if self.value_norm or self.value_dim != self.head_dim:
+            qkv = ops.value_norm_pad(qkv, H, G, self.head_dim, self.value_dim, self.eps, self.value_norm)
+        rot = self.position.rotary()
+        q, k = ops.qk_norm_rope(qkv, self.q_norm, self.k_norm, self.norm_eps, *(rot or (0, 1.0)), step, cache, H, G, D, True, False, True)
+        if rot is None:
+            q, k = self.position.apply(q, k, step.positions, step)
+        v = qkv[:, (H + G) * D:(H + 2 * G) * D]
+        step.drafted.append((k, v, cache.group, cache.pages))
+        return self._output(ops.tree_attention(q, k, v, step, cache, H, G, D, self.scale, self.window), ops)
+
     def forward(self, x, step, cache, write_cache=True):
+        if getattr(step, "tree_mask", None) is not None:
+            return self._forward_tree(x, step, cache, write_cache)
         if self.prepared:
             return self._forward_prepared(x, step, cache, write_cache)
         ops = step.ops
