@@ -254,26 +254,29 @@ struct CommitArgs {
 template <typename C> __global__ void __launch_bounds__(COMMIT_THREADS) commit_drafts_kernel(const CommitArgs a) {
     pdl_trigger();
     pdl_wait();
-    const int s = blockIdx.x, per_head = a.head_bytes / (int)sizeof(C), per_row = a.kv_heads * per_head;
+    // (pieces are numbered in 32 bits: 64-bit divisions cost 1.3 of 10.5 us for 640 rows of six layers, 4 KB each)
+    const int s = blockIdx.x;
+    const unsigned per_head = a.head_bytes / (unsigned)sizeof(C), per_row = a.kv_heads * per_head;
     int count = a.counts[s];
     if (count > a.most) {
         if (threadIdx.x == 0) zai_raise(a.status, ZAI_ST_ROWS);
         count = a.most;
     }
     const int first = a.cu[s];
-    const long long total = (long long)max(count, 0) * 2 * per_row;
-    const long long at0 = (long long)blockIdx.z * COMMIT_THREADS * COMMIT_ITEMS + threadIdx.x;
+    const unsigned total = (unsigned)max(count, 0) * 2 * per_row;
+    const unsigned at0 = blockIdx.z * (COMMIT_THREADS * COMMIT_ITEMS) + threadIdx.x;
+    if (at0 >= total) return;
     C piece[COMMIT_ITEMS];
     char* to[COMMIT_ITEMS];
 #pragma unroll
     for (int u = 0; u < COMMIT_ITEMS; ++u) {
-        const long long e = at0 + (long long)u * COMMIT_THREADS;
+        const unsigned e = at0 + u * COMMIT_THREADS;
         to[u] = nullptr;
         if (e >= total) continue;
-        const int i = (int)(e / (2 * per_row)), in_row = (int)(e - (long long)i * 2 * per_row);
-        const int which = in_row >= per_row, x = in_row - which * per_row, head = x / per_head, part = x - head * per_head;
+        const unsigned i = e / (2 * per_row), in_row = e - i * 2 * per_row, which = in_row >= per_row, x = in_row - which * per_row;
+        const unsigned head = x / per_head, part = x - head * per_head;
         const int row = a.path[(size_t)s * a.most + i];
-        if ((unsigned)row >= (unsigned)a.N || first < 0 || first + i >= a.N) {
+        if ((unsigned)row >= (unsigned)a.N || first < 0 || first + (int)i >= a.N) {
             zai_raise(a.status, ZAI_ST_ROWS);
             continue;
         }
@@ -307,6 +310,7 @@ ZAI_API int zai_commit_drafts(void* pages, const void* k, const void* v, long lo
     // pieces of 16 bytes where every row and head starts on one, else element by element
     const bool wide = !(((uintptr_t)pages | (uintptr_t)k | (uintptr_t)v) & 15) && !((a.k_plane | a.v_plane | a.k_row | a.v_row | head_bytes) & 15);
     const int size = wide ? 16 : es;
+    if ((long long)most * 2 * kv_heads * (head_bytes / size) > 0x3fffffffll) return ZAI_BAD_SIZE;
     const long long items = (long long)most * 2 * kv_heads * (head_bytes / size), per_block = COMMIT_THREADS * COMMIT_ITEMS;
     const long long z = (items + per_block - 1) / per_block;
     if (z > 65535) return ZAI_BAD_SIZE;

@@ -1324,19 +1324,18 @@ def token_logprobs(logits, tokens, top=0, blocks=0):
     top = int(top)
     if not logits.is_cuda or logits.stride(1) != 1 and V > 1 or logits.stride(0) < V and R > 1:
         raise KernelError("token_logprobs: logits are rows of contiguous values on a CUDA device")
-    if tokens.dtype != torch.int32 or tokens.shape != (R,) or not tokens.is_contiguous() or tokens.device != logits.device:
+    if tokens.dtype is not torch.int32 or tokens.shape != (R,) or not tokens.is_contiguous() or tokens.get_device() != logits.get_device():
         raise KernelError("token_logprobs: the tokens are int32, one for each row of logits, on the logits' device")
     if not 0 <= top <= min(32, V):
         raise KernelError(f"token_logprobs: {top} alternatives of {V} tokens; at most 32")
-    dev = logits.device
-    out = TokenLogprobs(logits.new_empty((R,), dtype=torch.float32), logits.new_empty((R,), dtype=torch.float32), torch.empty_like(tokens),
-                        tokens.new_empty((R, top)), logits.new_empty((R, top), dtype=torch.float32))
+    lp = logits.new_empty((R,), dtype=torch.float32)
+    out = TokenLogprobs(lp, torch.empty_like(lp), torch.empty_like(tokens), tokens.new_empty((R, top)), lp.new_empty((R, top)))
     if R == 0:
         return out
-    _on_current(dev, "token_logprobs")
+    status, sms, stream = _place(logits.get_device(), "token_logprobs")
     _check(_fn("logprobs", "zai_token_logprobs")(
-        out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), out[3].data_ptr(), out[4].data_ptr(), logits.data_ptr(), _dt(logits),
-        logits.stride(0), tokens.data_ptr(), R, V, top, int(blocks), _sm_count(dev), _status_ptr(dev), _stream()), "token_logprobs")
+        lp.data_ptr(), out[1].data_ptr(), out[2].data_ptr(), out[3].data_ptr(), out[4].data_ptr(), logits.data_ptr(), _dt(logits), logits.stride(0),
+        tokens.data_ptr(), R, V, top, int(blocks), sms, status, stream), "token_logprobs")
     return out
 
 
@@ -1356,27 +1355,29 @@ class StepLayout(NamedTuple):
 
 
 def _int32(what, *tensors):
-    """The device of contiguous int32 tensors that lie on one."""
+    """The number of the CUDA device on which these contiguous int32 tensors lie."""
     index = tensors[0].get_device()
     for t in tensors:
         if t.dtype is not torch.int32 or t.get_device() != index or index < 0 or not t.is_contiguous():
             raise KernelError(f"{what}: contiguous int32 tensors on one CUDA device are taken")
-    return tensors[0].device
+    return index
 
 
-def _on_current(device, what):
-    if device.index != torch.cuda.current_device():
-        raise KernelError(f"{what}: the tensors lie on {device}, the current device is cuda:{torch.cuda.current_device()}")
+_places = {}
 
 
-_sms = {}
-
-
-def _sm_count(device) -> int:
-    n = _sms.get(device.index)
-    if n is None:
-        n = _sms[device.index] = torch.cuda.get_device_properties(device).multi_processor_count
-    return n
+def _place(index, what):
+    """The status word, the SMs and the current stream of a device, which is to be the current one."""
+    current = torch.cuda.current_device()
+    if index != current:
+        raise KernelError(f"{what}: the tensors lie on cuda:{index}, the current device is cuda:{current}")
+    place = _places.get(index)
+    if place is None:
+        dev = torch.device("cuda", index)
+        place = _places[index] = (_status_ptr(dev), torch.cuda.get_device_properties(dev).multi_processor_count)
+    if _stream_handle is not None:
+        return place[0], place[1], _stream_handle
+    return place[0], place[1], torch.cuda.current_stream().cuda_stream if _raw_stream is None else _raw_stream(index)
 
 
 @_timed("step tables")
@@ -1386,20 +1387,20 @@ def step_layout(q_lens, ctx_lens, slots, page_rows, page_size, n_rows, width, pa
     of a block table.  `parents` [n_rows]: the rows are trees of drafted tokens of at most `tree_rows` rows each, and a row hangs on
     this row of its own span (-1: on none); a row's position is then its request's length plus its depth, and `tree_mask` holds
     its ancestors and itself.  Rows behind the last span belong to a span of no request: the null page, slot -1, nothing seen."""
-    dev = _int32("step_layout", q_lens, ctx_lens, slots, page_rows, *(() if parents is None else (parents,)))
+    index = _int32("step_layout", q_lens, ctx_lens, slots, page_rows, *(() if parents is None else (parents,)))
     S, N, width, tree_rows = q_lens.numel(), int(n_rows), int(width), int(tree_rows) if parents is not None else 0
     if ctx_lens.shape != q_lens.shape or slots.shape != q_lens.shape or q_lens.dim() != 1 or page_rows.dim() != 2:
         raise KernelError("step_layout: one length, one context and one slot a request, and the slots' block tables as rows")
     if parents is not None and (parents.shape != (N,) or not 1 <= tree_rows <= MAX_TREE_ROWS):
         raise KernelError(f"step_layout: a parent for each of the step's rows, and trees of 1 to {MAX_TREE_ROWS} rows")
-    _on_current(dev, "step_layout")
+    status, _, stream = _place(index, "step_layout")
     words = (tree_rows + 31) // 32
     sizes = (S + 2, S + 1, N, N, N, (S + 1) * width, N * words)
     parts = q_lens.new_empty((sum(sizes),)).split_with_sizes(sizes)
     p = [t.data_ptr() for t in parts]
     _check(_fn("drafts", "zai_step_layout")(
         *p, q_lens.data_ptr(), ctx_lens.data_ptr(), slots.data_ptr(), page_rows.data_ptr(), _ptr(parents), S, N, width, page_rows.shape[1],
-        page_rows.shape[0], int(page_size), tree_rows, words, _status_ptr(dev), _stream()), "step_layout")
+        page_rows.shape[0], int(page_size), tree_rows, words, status, stream), "step_layout")
     return StepLayout(*parts[:5], parts[5].view(S + 1, width), parts[6].view(N, words) if words else None)
 
 
@@ -1417,11 +1418,11 @@ def tree_attention(q, k, v, step, cache, heads, kv_heads, head_dim, scale, windo
     pages, bt, mask, cu_q, ctx_lens, positions = cache.pages, cache.block_table, step.tree_mask, step.cu_q, step.ctx_lens, step.positions
     if mask is None:
         raise KernelError("tree_attention: the step's rows are no trees (no tree_mask)")
-    dev = _int32("tree_attention", mask, bt, cu_q, ctx_lens, positions)
+    index = _int32("tree_attention", mask, bt, cu_q, ctx_lens, positions)
     if q.shape != (N, H * D) or k.shape != (N, G * D) or v.shape != (N, G * D):
         raise KernelError(f"tree_attention: q, k and v are rows of {H}, {G} and {G} heads of {D}")
     (qs, q1), (ks, k1), (vs, v1) = q.stride(), k.stride(), v.stride()
-    index, dtype = mask.get_device(), q.dtype
+    dtype = q.dtype
     if (q1 != 1 or k1 != 1 or v1 != 1 or k.dtype is not dtype or v.dtype is not dtype or pages.dtype is not dtype or q.get_device() != index
             or k.get_device() != index or v.get_device() != index or pages.get_device() != index or not pages.is_contiguous()
             or pages.shape[1:] != (2, G, cache.page_size, D) or N != step.n_tokens or mask.dim() != 2 or mask.shape[0] != N
@@ -1435,7 +1436,7 @@ def tree_attention(q, k, v, step, cache, heads, kv_heads, head_dim, scale, windo
     out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((N, H * D))
     if N == 0 or S == 0:
         return out
-    _on_current(dev, "tree_attention")
+    status, sms, stream = _place(index, "tree_attention")
     group, most = H // G, max(int(step.max_q_len), 1)
     qp, kp, vp, pp = q.data_ptr(), k.data_ptr(), v.data_ptr(), pages.data_ptr()
     mma = (q.dtype == torch.bfloat16 and impl != "general" and bool(_fn("tree_attention", "zai_tree_attention_mma_supports")(D))
@@ -1451,11 +1452,10 @@ def tree_attention(q, k, v, step, cache, heads, kv_heads, head_dim, scale, windo
     if impl == "tcgen05" and not tc:
         raise KernelError("tree_attention: the tcgen05 kernel takes bfloat16 heads of 64 or 128 on 16-byte boundaries, trees of at most 128 rows, no window")
     if tc:
-        blocks = _sm_count(dev)
-        parts = q.new_empty((blocks * _fn("tree_attention_tc", "zai_tree_attention_tc_part")(D),), dtype=torch.float32)
+        parts = q.new_empty((sms * _fn("tree_attention_tc", "zai_tree_attention_tc_part")(D),), dtype=torch.float32)
         _check(_fn("tree_attention_tc", "zai_tree_attention_tc")(
             out.data_ptr(), qp, qs, kp, ks, vp, vs, pp, bt.data_ptr(), bt.shape[1], cu_q.data_ptr(), ctx_lens.data_ptr(), mask.data_ptr(), mask.shape[1],
-            S, N, blocks, cache.page_size, pages.shape[0], H, G, D, scale, parts.data_ptr(), _status_ptr(dev), _stream()), "tree_attention (tcgen05)", 2)
+            S, N, sms, cache.page_size, pages.shape[0], H, G, D, scale, parts.data_ptr(), status, stream), "tree_attention (tcgen05)", 2)
         return out
     if mma:
         pairs = 16
@@ -1470,7 +1470,7 @@ def tree_attention(q, k, v, step, cache, heads, kv_heads, head_dim, scale, windo
         splits, keys = 1, width if window is None else min(width, int(window))
         while splits < 16 and splits * 64 < keys and tiles * G * splits < 256:
             splits *= 2
-    tail = (tiles, int(splits), cache.page_size, pages.shape[0], H, G, D, scale, int(window or 0), _status_ptr(dev), _stream())
+    tail = (tiles, int(splits), cache.page_size, pages.shape[0], H, G, D, scale, int(window or 0), status, stream)
     if mma:
         _check(_fn("tree_attention", "zai_tree_attention_mma")(
             out.data_ptr(), qp, qs, kp, ks, vp, vs, pp, bt.data_ptr(), bt.shape[1], cu_q.data_ptr(), ctx_lens.data_ptr(), positions.data_ptr(),
@@ -1496,19 +1496,19 @@ def accept_drafts(choices, tokens, parents, step, most):
     [N] int32) is the one chosen there (`choices` [N] int32, from `argmax` or `sample` on the rows' logits) is accepted and becomes
     the current one.  `parents` as in `step_layout`; a span has at most `most` rows.  S accepted paths, the tokens chosen along
     them, and the requests' lengths with the accepted rows."""
-    dev = _int32("accept_drafts", choices, tokens, parents, step.cu_q, step.ctx_lens)
+    index = _int32("accept_drafts", choices, tokens, parents, step.cu_q, step.ctx_lens)
     N, S, most = choices.numel(), step.cu_q.numel() - 1, int(most)
     if tokens.shape != choices.shape or parents.shape != choices.shape or choices.dim() != 1 or step.ctx_lens.numel() != S:
         raise KernelError("accept_drafts: a choice, a token and a parent a row, a length a span")
     if not 1 <= most <= MAX_TREE_ROWS:
         raise KernelError(f"accept_drafts: trees have 1 to {MAX_TREE_ROWS} rows")
-    _on_current(dev, "accept_drafts")
+    status, _, stream = _place(index, "accept_drafts")
     counts, ctx, path = torch.empty_like(step.ctx_lens), torch.empty_like(step.ctx_lens), choices.new_empty((S, most))
     chosen = torch.empty_like(path)
     if S:
         _check(_fn("drafts", "zai_accept_drafts")(
             counts.data_ptr(), path.data_ptr(), chosen.data_ptr(), ctx.data_ptr(), choices.data_ptr(), tokens.data_ptr(), parents.data_ptr(),
-            step.cu_q.data_ptr(), step.ctx_lens.data_ptr(), S, N, most, _status_ptr(dev), _stream()), "accept_drafts")
+            step.cu_q.data_ptr(), step.ctx_lens.data_ptr(), S, N, most, status, stream), "accept_drafts")
     return AcceptedDrafts(counts, path, chosen, ctx)
 
 
@@ -1517,7 +1517,7 @@ def commit_drafts(k, v, path, counts, step, pages):
     """Keys and values of accepted rows into the cache: the i-th row of `path` [S, most] (the first `counts` of a request's) goes to
     `step.kv_slots[step.cu_q[s] + i]`.  `pages` [pages, 2, kv_heads, page_size, head_dim] with k and v [N, kv_heads * head_dim], or
     the planes of several layers [L, pages, ...] with [L, N, ...]; rows may lie apart (columns of a projection)."""
-    dev = _int32("commit_drafts", path, counts, step.cu_q, step.kv_slots)
+    index = _int32("commit_drafts", path, counts, step.cu_q, step.kv_slots)
     if pages.dim() not in (5, 6) or k.dim() != pages.dim() - 3:
         raise KernelError("commit_drafts: pages of one layer with rows, or planes of several layers with as many sets of rows")
     planes = pages.shape[0] if pages.dim() == 6 else 1
@@ -1527,16 +1527,16 @@ def commit_drafts(k, v, path, counts, step, pages):
     S = counts.numel()
     if (two != 2 or tuple(k.shape) != want or tuple(v.shape) != want or k.dtype != pages.dtype or v.dtype != pages.dtype
             or not pages.is_contiguous() or k.stride(-1) != 1 or v.stride(-1) != 1 or path.dim() != 2 or path.shape[0] != S
-            or step.cu_q.numel() < S + 1 or step.kv_slots.numel() != N or any(t.device != dev for t in (k, v, pages))):
+            or step.cu_q.numel() < S + 1 or step.kv_slots.numel() != N or k.get_device() != index or v.get_device() != index or pages.get_device() != index):
         raise KernelError("commit_drafts: operands do not fit together")
-    _on_current(dev, "commit_drafts")
+    status, _, stream = _place(index, "commit_drafts")
     if S == 0 or N == 0 or planes == 0 or path.shape[1] == 0:
         return
     k_plane, v_plane = (k.stride(0), v.stride(0)) if pages.dim() == 6 else (0, 0)
     _check(_fn("drafts", "zai_commit_drafts")(
         pages.data_ptr(), k.data_ptr(), v.data_ptr(), k_plane, v_plane, k.stride(-2), v.stride(-2), path.data_ptr(), counts.data_ptr(),
-        step.cu_q.data_ptr(), step.kv_slots.data_ptr(), _dt(k), S, N, path.shape[1], planes, G, D, page_size, num_pages, _status_ptr(dev),
-        _stream()), "commit_drafts")
+        step.cu_q.data_ptr(), step.kv_slots.data_ptr(), _dt(k), S, N, path.shape[1], planes, G, D, page_size, num_pages, status,
+        stream), "commit_drafts")
 
 
 # ----------------------------------------------------------------------------- recurrent mixers and what goes with them
