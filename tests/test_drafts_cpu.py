@@ -186,3 +186,21 @@ def test_wrappers_refuse_tensors_off_the_device():
                  lambda: ops.accept_drafts(i, i, i, step, 2), lambda: ops.commit_drafts(x, x, i.view(3, 1), i, step, cache.pages)):
         with pytest.raises(ops.KernelError):
             call()
+
+
+def test_a_refused_score_or_choice_leaves_nothing_behind(model_dir):
+    eng = Engine(model_dir, "float32", max_num_seqs=2, max_batched_tokens=7, max_model_len=64, page_size=4, device="cpu", ops=ref_ops)
+    for prompts, top in (([[1, 2, 61]], 0), ([[1] * 9 + [-1]], 0), ([[1, 2]], 33), ([[1, 2]], -1), ([[1, 1 << 40]], 0)):
+        with pytest.raises(ValueError):
+            eng.score(prompts, top=top)
+    runner = eng.runner
+    assert not runner.processed
+    runner.add_request("a")
+    runner.step([("a", [1, 2, 3], [2])])
+    for choose in (lambda x: x.argmax(-1)[:1], lambda x: x.argmax(-1, keepdim=True)):
+        with pytest.raises(ValueError):
+            runner.verify([("a", [4, 5], [-1, 0])], choose)
+    assert runner.processed["a"] == 3
+    assert len(runner.verify([("a", [4, 5], [-1, 0])])[0]) in (1, 2)
+    runner.end_request("a")
+    runner.cache.check()

@@ -673,3 +673,87 @@ def test_layout_serves_the_kernels_that_are_there(tree_models):
     got = o.tree_attention(q, k, v, step, SimpleNamespace(pages=old, block_table=chain.block_tables, page_size=ps), H, G, D, 0.125)
     # (two kernels that each round the weights and the result to bfloat16: 2 (2^-8 sum p|v| + 2^-8 |o|), |v| < 6)
     assert float((got.float() - outs[0][1].float()).abs().max()) <= 4 * 2.0 ** -8 * float(v.float().abs().max())
+
+
+# ------------------------------------------------------------------------------------------------ lengths near the type's end, padded steps
+@pytest.mark.parametrize("dtype,impl", [(F32, None), (BF16, "general"), (BF16, "mma"), (BF16, "tcgen05")])
+@pytest.mark.parametrize("ctx", [2 ** 31 - 1, 2 ** 31 - 100, 2 ** 30])
+def test_lengths_beyond_the_block_table_raise_the_status_word(dtype, impl, ctx):
+    """What lies beyond a block table's row has no page; the other requests' rows come out as they do without it."""
+    o = ops()
+    q, k, v, step, cache, _ = make_tree_step([3, 4], [40, 30], 8, 2, 64, 16, dtype, 3, poison=0.0)
+    want = o.tree_attention(q, k, v, step, cache, 8, 2, 64, 0.125, impl=impl)
+    assert o.read_status() == 0
+    step.ctx_lens = ints([ctx, 30])
+    got = o.tree_attention(q, k, v, step, cache, 8, 2, 64, 0.125, impl=impl)
+    assert o.read_status() == 16
+    tol = 2e-5 if dtype == F32 else 2.0 ** -6                  # (another share of the keys may go to other blocks: two roundings of weights and result)
+    assert float((got[3:] - want[3:]).abs().max()) <= tol * float(v.float().abs().max())
+
+
+def test_tables_of_lengths_near_the_types_end_raise_the_status_word():
+    o, most = ops(), 2 ** 31 - 1
+    rows = torch.arange(1, 41, dtype=torch.int32, device="cuda").view(4, 10)
+    for ctx in (most, most - 1, 2 ** 30):
+        lay = o.step_layout(ints([3, 2]), ints([ctx, 5]), ints([0, 1]), rows, 4, 6, 10, ints([-1, 0, 0, -1, 0, -1]), 3)
+        assert o.read_status() == 16
+        assert lay.kv_slots.tolist() == [-1, -1, -1, int(rows[1, 1]) * 4 + 1, int(rows[1, 1]) * 4 + 2, -1]
+    one = ints([0, 0, 0, 0])
+    for cu in ([2, most], [-3, 4], [most, most], [3, 1], [-most - 1, most]):
+        step = SimpleNamespace(cu_q=ints(cu), ctx_lens=ints([7]), kv_slots=ints([4, 5, 6, 7]))
+        got = o.accept_drafts(one, one, ints([-1, 0, 1, 2]), step, 4)
+        assert got.counts.tolist() == [0] and got.path.tolist() == [[-1] * 4] and got.ctx_lens.tolist() == [7] and o.read_status() == 32
+    pages, kv = torch.zeros((4, 2, 1, 4, 8), device="cuda"), torch.ones((4, 8), device="cuda")
+    for first in (most, -1, -most - 1, 3):
+        step = SimpleNamespace(cu_q=ints([first, 4]), ctx_lens=ints([7]), kv_slots=ints([4, 5, 6, 7]))
+        o.commit_drafts(kv, kv, ints([[0, 1, 2]]), ints([3]), step, pages)
+        assert o.read_status() == 32 and float(pages.sum()) == (16 if first == 3 else 0)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("spare", [1, 40, 200])
+def test_rows_of_no_request_see_nothing(dtype, spare):
+    """A step of fixed size: the rows behind the last tree are a span of no request, longer than any tree; they come out as zeros."""
+    o, H, G, D, ps = ops(), 8, 2, 64, 16
+    q, k, v, step, cache, parents = make_tree_step([5, 0, 9], [700, 3, 31], H, G, D, ps, dtype, 6)
+    want = o.tree_attention(q, k, v, step, cache, H, G, D, 0.125)
+    n, N = 14, 14 + spare
+    wide = [torch.cat([x, torch.randn((spare, x.shape[1]), device="cuda").to(dtype)]) for x in (q, k, v)]
+    lay = o.step_layout(ints([5, 0, 9]), step.ctx_lens, ints([0, 1, 2]), cache.block_table, ps, N, cache.block_table.shape[1],
+                        ints([p for ps_ in parents for p in ps_] + [-1] * spare), 9)
+    padded = SimpleNamespace(cu_q=lay.cu_q, ctx_lens=lay.ctx_lens, positions=lay.positions, tree_mask=lay.tree_mask, n_seqs=4, n_tokens=N, max_q_len=max(9, spare))
+    got = o.tree_attention(*wide, padded, SimpleNamespace(pages=cache.pages, block_table=lay.block_tables, page_size=ps), H, G, D, 0.125)
+    assert o.read_status() == 0 and not got[n:].any()
+    assert torch.equal(lay.positions[:n], step.positions) and torch.equal(lay.tree_mask[:n], step.tree_mask)
+    assert float((got[:n].float() - want.float()).abs().max()) <= (1e-5 if dtype == F32 else 2.0 ** -6) * float(v.float().abs().max())
+
+
+def test_scores_beside_requests_that_are_served(tree_models):
+    """A prompt scored while a decode step is on its way changes neither that step's requests nor its own log probabilities."""
+    from zig_ai_b200.engine import Engine
+    d, cfg = tree_models["A"]
+    g = random.Random(12)
+    prompts = [[g.randrange(cfg["vocab_size"]) for _ in range(n)] for n in (17, 5)]
+    scored = [[g.randrange(cfg["vocab_size"]) for _ in range(n)] for n in (40, 2, 1)]
+
+    def engine():
+        return Engine(d, "float32", max_num_seqs=4, max_batched_tokens=32, max_model_len=128, page_size=16)
+    alone = engine()
+    want_out, want_score = alone.generate(prompts, max_new_tokens=12), alone.score(scored, top=2)
+    eng = engine()
+    from zig_ai_b200.sampling import SamplingParams
+    ids = [eng.add_request(p, SamplingParams(temperature=0.0, max_new_tokens=12)) for p in prompts]
+    done, n = {}, 0
+    while eng.has_work():
+        for r in eng.step():
+            done[r.request_id] = r.output
+        n += 1
+        if n in (3, 5):
+            got = eng.score(scored, top=2)
+            for a, b in zip(got, want_score):
+                assert [(e["token"], e["rank"], [t for t, _ in e["top"]]) for e in a] == [(e["token"], e["rank"], [t for t, _ in e["top"]]) for e in b]
+                assert all(abs(x["logprob"] - y["logprob"]) < 1e-4 for x, y in zip(a, b))
+    for r in eng.flush():
+        done[r.request_id] = r.output
+    assert [done[i] for i in ids] == want_out
+    eng.runner.cache.check()

@@ -125,9 +125,10 @@ __global__ void __launch_bounds__(LAYOUT_THREADS) step_layout_kernel(const Layou
             s = lo;
             const int first = cu[s], i = r - first, c = max(a.ctx[s], 0);
             const int place = zai_checked_slot(a.slots[s], a.n_slots, a.status);
-            pos = c + i;
-            const int j = pos / a.page_size;
-            if (j >= a.width || j >= a.row_width || pos < 0) zai_raise(a.status, ZAI_ST_POSITION);
+            const unsigned at_most = (unsigned)c + i, page_index = at_most / a.page_size;     // (unsigned: a length near the type's end must not wrap)
+            const int j = (int)min(page_index, 0x7fffffffu);
+            pos = (int)at_most;
+            if (j >= a.width || j >= a.row_width || at_most > 0x7fffffffu) zai_raise(a.status, ZAI_ST_POSITION);
             else {
                 const int page = a.page_rows[(size_t)place * a.row_width + j];
                 const long long at = (long long)page * a.page_size + (pos - j * a.page_size);
@@ -151,7 +152,7 @@ __global__ void __launch_bounds__(LAYOUT_THREADS) step_layout_kernel(const Layou
                         cur = up;
                         ++depth;
                     }
-                    pos = c + depth;
+                    pos = (int)((unsigned)c + depth);
                 }
             }
         } else {
@@ -198,12 +199,10 @@ __global__ void __launch_bounds__(ACCEPT_WARPS * 32) accept_drafts_kernel(int* c
     pdl_trigger();
     pdl_wait();
     if (s >= S) return;
-    int a = cu[s], n = cu[s + 1] - a;
-    const int cached = ctx[s];
-    if (a < 0 || n < 0 || a + n > N) {
-        if (lane == 0) zai_raise(status, ZAI_ST_ROWS);
-        n = 0;
-    }
+    const int a = cu[s], end = cu[s + 1], cached = ctx[s];
+    const bool inside = a >= 0 && end >= a && end <= N;
+    int n = inside ? end - a : 0;
+    if (!inside && lane == 0) zai_raise(status, ZAI_ST_ROWS);
     if (n > most) {                                            // a span of more rows than a tree may have: what is behind them is not looked at
         if (lane == 0) zai_raise(status, ZAI_ST_TREE);
         n = most;
@@ -276,7 +275,7 @@ template <typename C> __global__ void __launch_bounds__(COMMIT_THREADS) commit_d
         const unsigned i = e / (2 * per_row), in_row = e - i * 2 * per_row, which = in_row >= per_row, x = in_row - which * per_row;
         const unsigned head = x / per_head, part = x - head * per_head;
         const int row = a.path[(size_t)s * a.most + i];
-        if ((unsigned)row >= (unsigned)a.N || first < 0 || first + (int)i >= a.N) {
+        if ((unsigned)row >= (unsigned)a.N || first < 0 || (unsigned)first + i >= (unsigned)a.N) {
             zai_raise(a.status, ZAI_ST_ROWS);
             continue;
         }

@@ -469,7 +469,7 @@ static int launch_logprobs(float* logprobs, float* entropy, int* ranks, int* top
 ZAI_API int zai_token_logprobs(float* logprobs, float* entropy, int* ranks, int* top_ids, float* top_logprobs, const void* logits, int dtype,
                                long long stride, const int* targets, int R, int V, int top, int blocks, int sms, int* status,
                                cudaStream_t stream) {
-    if (R < 1 || V < 1 || V > 0x7fffffff - 2 * LP_THREADS * LP_ROUND || R > 0x7fffffff / 16 || top < 0 || top > 32 || top > V || blocks < 0 || blocks > 16 ||
+    if (R < 1 || V < 1 || V > 0x7fffffff - 8 * LP_THREADS * LP_ROUND || R > 0x7fffffff / 16 || top < 0 || top > 32 || top > V || blocks < 0 || blocks > 16 ||
         (blocks & (blocks - 1)))
         return ZAI_BAD_SIZE;
     if (blocks == 0)

@@ -27,6 +27,7 @@ struct TreeArgs {
     const int *table, *cu, *ctx, *positions;
     const unsigned* mask;
     int table_width, words, S, N, page_size, page_shift, num_pages, H, G, D, window;     // page_shift: of a page size that is a power of two, else -1
+    int reach;                                                 // positions that a block table's row holds
     float scale;
     int* status;
 };
@@ -70,6 +71,10 @@ __device__ __forceinline__ Tile find_tile(const TreeArgs& a, int number, int M, 
             t.n = __shfl_sync(0xffffffffu, n, w);
             t.pair0 = (number - __shfl_sync(0xffffffffu, upto - tiles, w)) * M;
             t.ctx = max(a.ctx[t.s], 0);
+            if (t.ctx > a.reach) {                             // (what is beyond has no page)
+                zai_raise(a.status, ZAI_ST_POSITION);
+                t.ctx = a.reach;
+            }
             if (!last) return t;
             if (__shfl_sync(0xffffffffu, upto, 31) > number + 1) {
                 zai_raise(a.status, ZAI_ST_TREE);
@@ -654,6 +659,11 @@ __global__ void __launch_bounds__(32 * WM * WN) tree_attention_mma_kernel(const 
 }
 
 // ---------------------------------------------------------------------------------------------------- launching
+// Positions that a row of `table_width` pages holds; 2^30 at most, so that sums of positions and rows stay within 32 bits.
+static int reach_of(int table_width, int page_size) {
+    const long long n = (long long)table_width * page_size;
+    return n > 0x3fffffffll ? 0x3fffffff : (int)n;
+}
 static int page_shift_of(int page_size) {
     int shift = 0;
     while ((1 << shift) < page_size) ++shift;
@@ -711,7 +721,7 @@ ZAI_API int zai_tree_attention_general(void* out, const void* q, long long q_str
         D < 1 || D > 512 || words < 1 || table_width < 1 || (long long)N * (H / G) > 0x3fffffff)
         return ZAI_BAD_SIZE;
     const TreeArgs a = {out, q, k, v, pages, q_stride, k_stride, v_stride, table, cu, ctx, positions, (const unsigned*)mask, table_width, words, S, N,
-                        page_size, page_shift_of(page_size), num_pages, H, G, D, window, scale, status};
+                        page_size, page_shift_of(page_size), num_pages, H, G, D, window, reach_of(table_width, page_size), scale, status};
     if (dtype == ZAI_BF16) return launch_general_cols<bf16, false>(a, tiles, splits, stream);
     if (dtype != ZAI_F32) return ZAI_BAD_DTYPE;
     const bool wide = !(((uintptr_t)k | (uintptr_t)v | (uintptr_t)pages) & 15) && !((k_stride | v_stride | D) & 3);
@@ -748,7 +758,7 @@ ZAI_API int zai_tree_attention_mma(void* out, const void* q, long long q_stride,
     if ((((uintptr_t)k | (uintptr_t)v | (uintptr_t)pages) & 15) || ((k_stride | v_stride) & 7) || ((uintptr_t)q & 3) || (q_stride & 1) || ((uintptr_t)out & 7))
         return ZAI_BAD_SIZE;
     const TreeArgs a = {out, q, k, v, pages, q_stride, k_stride, v_stride, table, cu, ctx, positions, (const unsigned*)mask, table_width, words, S, N,
-                        page_size, page_shift_of(page_size), num_pages, H, G, D, window, scale, status};
+                        page_size, page_shift_of(page_size), num_pages, H, G, D, window, reach_of(table_width, page_size), scale, status};
     switch (D) {
         case 32: return launch_mma_pairs<32>(a, pairs, tiles, splits, stream);
         case 64: return launch_mma_pairs<64>(a, pairs, tiles, splits, stream);

@@ -39,6 +39,7 @@ struct TtArgs {
     const unsigned* mask;
     int table_width, words, S, N, page_size, page_shift, num_pages, H, G;
     int group, dual_cost;               // query heads of a key/value head; what a tile that both turns work on costs
+    int reach;                          // positions that a block table's row holds
     float scale;
     float* parts;                       // [2 blocks][TT_UNIT][D]: O, then [2 blocks][TT_UNIT][2]: reference and sum, then [blocks] Cut
     int* status;
@@ -66,6 +67,10 @@ __device__ __forceinline__ Request request_of(const TtArgs& a, int s, bool say) 
     if (r.n > TT_ROWS) {
         if (say) zai_raise(a.status, ZAI_ST_TREE);
         r.n = TT_ROWS;
+    }
+    if (r.ctx > a.reach) {                                      // (what is beyond has no page)
+        if (say) zai_raise(a.status, ZAI_ST_POSITION);
+        r.ctx = a.reach;
     }
     r.tiles = (r.ctx + TT_KEYS - 1) / TT_KEYS + 1;
     const int pairs = r.n * a.group;
@@ -805,7 +810,8 @@ ZAI_API int zai_tree_attention_tc(void* out, const void* q, long long q_stride, 
         return ZAI_BAD_SIZE;
     int shift = 0;
     while ((1 << shift) < page_size) ++shift;
+    const long long reach = (long long)table_width * page_size;
     const TtArgs a = {(bf16*)out, (const bf16*)q, (const bf16*)k, (const bf16*)v, (const bf16*)pages, q_stride, k_stride, v_stride, table, cu, ctx,
-                      (const unsigned*)mask, table_width, words, S, N, page_size, shift, num_pages, H, G, H / G, 1, scale, parts, status};
+                      (const unsigned*)mask, table_width, words, S, N, page_size, shift, num_pages, H, G, H / G, 1, reach > 0x3fffffffll ? 0x3fffffff : (int)reach, scale, parts, status};
     return D == 64 ? launch_tree_tc<64>(a, blocks, stream) : launch_tree_tc<128>(a, blocks, stream);
 }

@@ -246,11 +246,15 @@ class Engine:
         behind the tokens before it (`logprob`), its `rank` among all tokens (0: the likeliest), the `entropy` there in nats, and the
         `top` (at most 32) likeliest tokens with their log probabilities (`top`, pairs).  Runs beside requests that are being
         served if slots and pages are free; prompts are cut into portions of `max_batched_tokens`."""
-        out = []
+        out, V = [], self.runner.model.vocab_size
+        if not 0 <= int(top) <= min(32, V):
+            raise ValueError(f"{top} alternatives of {V} tokens; at most 32")
         for k, prompt in enumerate(prompts):
             tokens, rid, entries = [int(t) for t in prompt], ("score", self._next_id, k), []
             if not 0 < len(tokens) <= self.max_model_len:
                 raise ValueError(f"a prompt of {len(tokens)} tokens cannot be scored; the model's length is {self.max_model_len}")
+            if not all(0 <= t < V for t in tokens):
+                raise ValueError(f"token ids {[t for t in tokens if not 0 <= t < V][:8]} are outside the vocabulary of {V}")
             self.runner.add_request(rid)
             try:
                 for a in range(0, len(tokens), self.scheduler.max_batched_tokens):

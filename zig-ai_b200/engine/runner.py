@@ -227,7 +227,10 @@ class ModelRunner:
         step, tokens, parents, layouts = lay_out_trees(ops, self.dtype, self.device, spans, [p for _, _, p in entries], tables, self.cache.page_size, n + pad)
         logits = self.model.forward(step, self.cache)
         choices = torch.zeros_like(tokens)
-        choices[:n] = (choose or ops.argmax)(logits)
+        chosen = (choose or ops.argmax)(logits)
+        if tuple(chosen.shape) != (n,):
+            raise StepError(f"{n} rows want a choice each, got {tuple(chosen.shape)}")
+        choices[:n] = chosen
         accepted = ops.accept_drafts(choices, tokens, parents, step, step.max_q_len)
         for k, v, group, pages in step.drafted:
             ops.commit_drafts(k, v, accepted.path, accepted.counts, layouts[group], pages)

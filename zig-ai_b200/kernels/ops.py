@@ -1389,6 +1389,8 @@ def step_layout(q_lens, ctx_lens, slots, page_rows, page_size, n_rows, width, pa
     its ancestors and itself.  Rows behind the last span belong to a span of no request: the null page, slot -1, nothing seen."""
     index = _int32("step_layout", q_lens, ctx_lens, slots, page_rows, *(() if parents is None else (parents,)))
     S, N, width, tree_rows = q_lens.numel(), int(n_rows), int(width), int(tree_rows) if parents is not None else 0
+    if N < 0 or width < 1 or int(page_size) < 1:
+        raise KernelError(f"step_layout: {N} rows, block tables of {width} pages of {page_size} positions")
     if ctx_lens.shape != q_lens.shape or slots.shape != q_lens.shape or q_lens.dim() != 1 or page_rows.dim() != 2:
         raise KernelError("step_layout: one length, one context and one slot a request, and the slots' block tables as rows")
     if parents is not None and (parents.shape != (N,) or not 1 <= tree_rows <= MAX_TREE_ROWS):
@@ -1410,8 +1412,11 @@ def tree_attention(q, k, v, step, cache, heads, kv_heads, head_dim, scale, windo
     rows of its own span whose bit stands in `step.tree_mask` [N, words] (int32; as `step_layout` makes it); keys and values of
     the step's rows are k and v [N, kv_heads * head_dim] (columns of the projection's rows are fine) and enter no page:
     `commit_drafts` caches those that are accepted.  `window`: of all these, the ones whose position is above the row's minus the
-    window (`step.positions`: ctx plus the row's depth).  A row that sees nothing gets zeros.  `impl`: "general" or "mma"; `splits`: how
-    many blocks share a tile's keys (None: by the sizes)."""
+    window (`step.positions`: ctx plus the row's depth).  A row that sees nothing gets zeros.  `step.max_q_len` bounds all spans, that of
+    no request among them; a longer one raises the status word.  `impl`: "general", "mma" or "tcgen05" (None: by the sizes); `splits`:
+    how many blocks share a tile's keys in the first two (None: by the sizes)."""
+    if impl not in (None, "general", "mma", "tcgen05"):
+        raise KernelError(f"tree_attention: no kernel {impl!r}")
     N, H, G, D, S = q.shape[0], int(heads), int(kv_heads), int(head_dim), step.n_seqs
     if G < 1 or H % G:
         raise KernelError(f"tree_attention: {H} query heads cannot share {G} key/value heads evenly")
