@@ -26,9 +26,11 @@
 #define TT_UNIT 256                     // pairs of a unit
 #define TT_ROWS 128                     // rows of a tree: one tile of keys
 #define TT_SOFTMAX 8
-#define TT_LOADERS 4
+#define TT_LOADERS 2                    // (twelve warps leave a thread 168 registers; with four loaders, 128)
+#define TT_SUB (TT_TILE / 32 / TT_LOADERS)      // groups of 32 rows of a tile that a loading warp copies
 #define TT_THREADS (32 * (TT_SOFTMAX + TT_LOADERS + 2))
 #define TT_LEAST 4                      // cost of a share: fewer blocks take part when there is less than this for each
+#define TT_EXTRA 3                      // cost of a unit beside its tiles (its queries, first scores and end)
 #define TT_LOG2E 1.4426950408889634f
 
 struct TtArgs {
@@ -38,10 +40,10 @@ struct TtArgs {
     const int *table, *cu, *ctx;
     const unsigned* mask;
     int table_width, words, S, N, page_size, page_shift, num_pages, H, G;
-    int group, dual_cost;               // query heads of a key/value head; what a tile that both turns work on costs
+    int group, dual_cost, unit_extra;   // query heads of a key/value head; what a tile that both turns work on costs, and a unit beside its tiles
     int reach;                          // positions that a block table's row holds
     float scale;
-    float* parts;                       // [2 blocks][TT_UNIT][D]: O, then [2 blocks][TT_UNIT][2]: reference and sum, then [blocks] Cut
+    float* parts;                       // [2 blocks][D / 4][TT_UNIT][4]: O, then [2 blocks][TT_UNIT][2]: reference and sum, then [blocks] Cut
     int* status;
 };
 
@@ -79,7 +81,7 @@ __device__ __forceinline__ Request request_of(const TtArgs& a, int s, bool say) 
     return r;
 }
 __device__ __forceinline__ long long cost_of(const TtArgs& a, const Request& r) {
-    return r.n ? (long long)a.G * r.tiles * ((long long)a.dual_cost * (r.row_units - 1) + r.last_cost) : 0;
+    return r.n ? a.G * (r.tiles * ((long long)a.dual_cost * (r.row_units - 1) + r.last_cost) + (long long)a.unit_extra * r.row_units) : 0;
 }
 __device__ __forceinline__ int divided(long long x, long long by) {      // (32-bit where both fit, which is nearly always)
     return (x | by) >> 31 ? (int)(x / by) : (int)((unsigned)x / (unsigned)by);
@@ -106,17 +108,20 @@ struct Cut { int first, pair0, pairs, head, b0, b1, spare[2]; };
 struct Place { int row, head, w; long long unit, per; };
 __device__ __forceinline__ Place place_of(const TtArgs& a, const Request& r, long long base, long long pos) {
     const int w = a.dual_cost;
-    const long long full = (long long)w * a.G * r.tiles;        // a row of full units
+    const long long full = a.G * ((long long)w * r.tiles + a.unit_extra);      // a row of full units
     Place p;
     p.row = min(divided(pos - base, full), r.row_units - 1);
     p.w = p.row + 1 < r.row_units ? w : r.last_cost;
-    p.per = (long long)p.w * r.tiles;
+    p.per = (long long)p.w * r.tiles + a.unit_extra;
     const long long row_base = base + p.row * full;
     p.head = divided(pos - row_base, p.per);
     p.unit = row_base + p.head * p.per;
     return p;
 }
-__device__ __forceinline__ int tiles_before(const Place& p, long long cost) { return (int)((cost - p.unit + p.w - 1) >> (p.w - 1)); }
+// (a unit's extra cost comes before its tiles')
+__device__ __forceinline__ int tiles_before(const TtArgs& a, const Place& p, long long cost) {
+    return (int)(max(cost - p.unit - a.unit_extra + p.w - 1, 0LL) >> (p.w - 1));
+}
 
 struct Segment {
     int s, first, n, ctx, pair0, pairs, head, tiles, from, upto;       // key tiles [from, upto) of the unit's `tiles`
@@ -142,7 +147,7 @@ struct Walk {
                 p.unit += p.per;
                 p.head = 0;
                 if (p.row + 1 == r.row_units) p.w = r.last_cost;
-                p.per = (long long)p.w * r.tiles;
+                p.per = (long long)p.w * r.tiles + a.unit_extra;
             } else {
                 p.unit += p.per;
                 do {                                            // (there is one: pos lies before the end)
@@ -150,11 +155,11 @@ struct Walk {
                 } while (r.n == 0 && s < a.S - 1);
                 p.row = p.head = 0;
                 p.w = r.row_units > 1 ? a.dual_cost : r.last_cost;
-                p.per = (long long)p.w * r.tiles;
+                p.per = (long long)p.w * r.tiles + a.unit_extra;
             }
             const long long stop = min(end, p.unit + p.per);
-            g.from = tiles_before(p, pos);
-            g.upto = tiles_before(p, stop);
+            g.from = tiles_before(a, p, pos);
+            g.upto = tiles_before(a, p, stop);
             pos = stop;
             if (g.from == g.upto) continue;
             g.s = s;
@@ -214,9 +219,7 @@ __device__ __forceinline__ void begin_walk(const TtArgs& a, int D, long long* sh
         if (pos < end) {
             const Request r = request_of(a, s, false);
             const Place p = place_of(a, r, base, pos);
-            const int b0 = shares.owner(p.unit);
-            int b1 = shares.owner(p.unit + p.per - 1);
-            if (tiles_before(p, shares.start(b1)) >= r.tiles) --b1;     // (half a tile's cost holds no tile)
+            const int b0 = shares.owner(p.unit + a.unit_extra), b1 = shares.owner(p.unit + p.per - p.w);     // the first tile's block and the last one's
             if (b0 < (int)blockIdx.x && (int)blockIdx.x <= b1) {
                 cut.first = r.first;
                 cut.pair0 = p.row * TT_UNIT;
@@ -243,6 +246,11 @@ __device__ __forceinline__ float2 tt_add2(float2 a, float2 b) {
         : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
     return d;
 }
+__device__ __forceinline__ float tt_max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ void tt_ld16_nowait(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
@@ -261,6 +269,10 @@ __device__ __forceinline__ void tt_arrive_landed(uint64_t* bar) {
 }
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
+// (a loader's waits are long ones: it naps between its tries, whose instructions the softmax warps would miss)
+__device__ __forceinline__ bool tt_wait_warp(uint64_t* bar, uint32_t parity, volatile int* failed) {
+    return __all_sync(0xffffffffu, at_mbar_wait<AT_NAP_NS>(bar, parity, failed));
+}
 // What the loaders and the other warps share.
 struct Pipe {
     unsigned char *q, *ring;
@@ -279,10 +291,10 @@ template <int KS, int VS> struct Ring {
     static __device__ __forceinline__ uint32_t v_round(int t) { return (t / VS) & 1; }
 };
 
-// The loading warps.  D: a head's columns; KS, VS: slots of the ring; QROWS: pairs that there is room for.
-template <int D, int KS, int VS, int QROWS>
+// The loading warps.  D: a head's columns; KS, VS: slots of the ring.
+template <int D, int KS, int VS>
 __device__ __forceinline__ void load_units(const TtArgs& a, const CUtensorMap* pages_map, Walk walk, const Pipe& pipe, int lw) {
-    constexpr int BLOCK = TT_TILE * 128, SLOT = D / 64 * BLOCK, CHUNKS = D / 8, QTILE = QROWS < TT_TILE ? QROWS : TT_TILE;
+    constexpr int BLOCK = TT_TILE * 128, SLOT = D / 64 * BLOCK, CHUNKS = D / 8;
     const int lane = threadIdx.x & 31, group = a.group;
     unsigned char *sQ = pipe.q, *ring = pipe.ring;
     uint64_t *full = pipe.full, *empty = pipe.empty, *q_full = pipe.q_full, *q_empty = pipe.q_empty;
@@ -291,12 +303,12 @@ __device__ __forceinline__ void load_units(const TtArgs& a, const CUtensorMap* p
     using R = Ring<KS, VS>;
     int count = 0, seg = 0;                                 // tiles begun
     bool ok = true;
-    auto copy_tile = [&](unsigned char* dst, const bf16* mine, int block) {       // rows of D values, this warp's 32, a row's start in each lane
+    auto copy_rows = [&](unsigned char* dst, const bf16* mine, int rows) {        // 32 rows of D values, the 32 rows-th of the tile, a row's start in each lane
 #pragma unroll
         for (int e = 0; e < CHUNKS; ++e) {
-            const int f = e * 32 + lane, r = f / CHUNKS, c = f % CHUNKS, row = lw * 32 + r;
+            const int f = e * 32 + lane, r = f / CHUNKS, c = f % CHUNKS, row = rows * 32 + r;
             const bf16* p = (const bf16*)__shfl_sync(0xffffffffu, (unsigned long long)mine, r);
-            cp_async16(dst + (c >> 3) * block + row * 128 + (((c & 7) ^ (row & 7)) << 4), p ? p + c * 8 : a.pages, p != nullptr);
+            cp_async16(dst + (c >> 3) * BLOCK + row * 128 + (((c & 7) ^ (row & 7)) << 4), p ? p + c * 8 : a.pages, p != nullptr);
         }
     };
     while (ok && walk.next(a, g)) {
@@ -312,8 +324,8 @@ __device__ __forceinline__ void load_units(const TtArgs& a, const CUtensorMap* p
             const int idx = (tile * TT_KEYS + lane * box) >> a.page_shift;
             return tile < whole && tile < g.upto && lane < boxes && idx < a.table_width ? table[idx] : -1;
         };
-        auto find = [&](int tile, const bf16*& kp, const bf16*& vp) {
-            const int node = lw * 32 + lane, key = tile * TT_KEYS + node;
+        auto find = [&](int tile, int rows, const bf16*& kp, const bf16*& vp) {
+            const int node = rows * 32 + lane, key = tile * TT_KEYS + node;
             kp = vp = nullptr;
             if (tile == g.tiles - 1) {
                 if (node < g.n) {
@@ -330,25 +342,27 @@ __device__ __forceinline__ void load_units(const TtArgs& a, const CUtensorMap* p
         bool have_q = false;
         auto queries = [&](bool wait) {
             const uint32_t parity = (seg & 1) ^ 1;
-            if (wait) ok = at_mbar_wait_warp(q_empty, parity, failed);
+            if (wait) ok = tt_wait_warp(q_empty, parity, failed);
             else if (!__all_sync(0xffffffffu, at_mbar_test(q_empty, parity))) return;
             if (!ok) return;
-            for (int h = 0; h < (QROWS > TT_TILE && g.dual() ? 2 : 1) && lw * 32 < QTILE; ++h) {
-                const int r = h * TT_TILE + lw * 32 + lane, p = g.pair0 + r;
-                copy_tile(sQ + h * SLOT, r < g.pairs ? a.q + (long long)(g.first + p / group) * a.q_stride + (g.head * group + p % group) * D : nullptr, QTILE * 128);
-            }
+            for (int h = 0; h < (g.dual() ? 2 : 1); ++h)
+#pragma unroll
+                for (int u = 0; u < TT_SUB; ++u) {
+                    const int r = h * TT_TILE + (lw * TT_SUB + u) * 32 + lane, p = g.pair0 + r;
+                    copy_rows(sQ + h * SLOT, r < g.pairs ? a.q + (long long)(g.first + p / group) * a.q_stride + (g.head * group + p % group) * D : nullptr, lw * TT_SUB + u);
+                }
             tt_arrive_landed(q_full);
             have_q = true;
         };
         int page = ask(g.from), next = -1;
-        const bf16 *kp = nullptr, *vp = nullptr;
+        const bf16 *kp[TT_SUB] = {}, *vp[TT_SUB] = {};
         for (int i = 0; i < 2 * (g.upto - g.from) && ok; count += i & 1, ++i) {
             const int slot = i & 1 ? R::v_slot(count) : R::k_slot(count), tile = g.from + (i >> 1);
             const uint32_t parity = (i & 1 ? R::v_round(count) : R::k_round(count)) ^ 1;
             if (!have_q) queries(i >= 2 * (KS < VS ? KS : VS) - 1);
             // (a slot that is in use may be one of this unit's own, which its queries free)
             if (ok && !have_q && !__all_sync(0xffffffffu, at_mbar_test(&empty[slot], parity))) queries(true);
-            if (ok) ok = at_mbar_wait_warp(&empty[slot], parity, failed);
+            if (ok) ok = tt_wait_warp(&empty[slot], parity, failed);
             if (!ok) break;
             unsigned char* dst = ring + (size_t)slot * SLOT;
             if (tile < whole) {
@@ -371,23 +385,29 @@ __device__ __forceinline__ void load_units(const TtArgs& a, const CUtensorMap* p
                 continue;
             }
             if (!(i & 1)) {
-                find(tile, kp, vp);
-                copy_tile(dst, kp, BLOCK);
+#pragma unroll
+                for (int u = 0; u < TT_SUB; ++u) {
+                    find(tile, lw * TT_SUB + u, kp[u], vp[u]);
+                    copy_rows(dst, kp[u], lw * TT_SUB + u);
+                }
             } else {
-                copy_tile(dst, vp, BLOCK);
                 bool bad = false;                           // is one of this lane's values, drafted ones, not finite?  (A look at memory: to wait for the
-                if (tile == g.tiles - 1 && vp) {            // copies would hold up the next unit's)
+#pragma unroll
+                for (int u = 0; u < TT_SUB; ++u) {          // copies would hold up the next unit's)
+                    copy_rows(dst, vp[u], lw * TT_SUB + u);
+                    if (tile != g.tiles - 1 || !vp[u]) continue;
                     uint4 x[CHUNKS];
 #pragma unroll
-                    for (int c = 0; c < CHUNKS; ++c) x[c] = *reinterpret_cast<const uint4*>(vp + c * 8);
+                    for (int c = 0; c < CHUNKS; ++c) x[c] = *reinterpret_cast<const uint4*>(vp[u] + c * 8);
 #pragma unroll
                     for (int c = 0; c < CHUNKS; ++c) bad |= at_not_finite(x[c]);
                 }
                 if (__any_sync(0xffffffffu, bad)) {         // zeros in their place (what a row sees is put right at its end)
                     cp_async_wait_all();
                     bool mine = false;
-                    for (int e = 0; e < CHUNKS; ++e) {
-                        const int f = e * 32 + lane, key = lw * 32 + f / CHUNKS, c = f % CHUNKS;
+                    __syncwarp();
+                    for (int e = 0; e < CHUNKS * TT_SUB; ++e) {
+                        const int f = e * 32 + lane, key = lw * TT_SUB * 32 + f / CHUNKS, c = f % CHUNKS;
                         unsigned char* at = dst + (c >> 3) * BLOCK + key * 128 + (((c & 7) ^ (key & 7)) << 4);
                         if (at_not_finite(*reinterpret_cast<const uint4*>(at))) {
                             mine = true;
@@ -485,7 +505,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attention_tc_kernel(const 
     if (failed_flag) {
         // (nothing to wait for)
     } else if (warp >= TT_SOFTMAX && warp < TT_SOFTMAX + TT_LOADERS) {
-        load_units<D, Shape::KS, Shape::VS, TT_UNIT>(a, &pages_map, walk, Pipe{sQ, ring, full, empty, q_full, q_empty, odd, failed}, warp - TT_SOFTMAX);
+        load_units<D, Shape::KS, Shape::VS>(a, &pages_map, walk, Pipe{sQ, ring, full, empty, q_full, q_empty, odd, failed}, warp - TT_SOFTMAX);
     } else if (warp >= TT_SOFTMAX + TT_LOADERS) {
         if (zai_elect()) {
             // ---- products, a warp a turn, half a tile's keys at a time: while one half is in the softmax, the other's P is multiplied and its buffer
@@ -603,7 +623,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attention_tc_kernel(const 
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
                         for (int j = 0; j < 32; j += 2)
-                            mx[(j >> 1) & 3] = fmaxf(mx[(j >> 1) & 3], fmaxf(__uint_as_float(x[i][j]), __uint_as_float(x[i][j + 1])));
+                                                        mx[(j >> 1) & 3] = tt_max3(mx[(j >> 1) & 3], __uint_as_float(x[i][j]), __uint_as_float(x[i][j + 1]));
                     // The reference is the first half's maximum, and moves when a later one exceeds it by 2^8: a weight keeps its 8 bits whatever the
                     // reference is, and the sum is that of the rounded weights, so what one key dominates stays exact.
                     const float most = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
@@ -629,19 +649,15 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attention_tc_kernel(const 
                     const float2 c2 = make_float2(c, c), minus = make_float2(m == -INFINITY ? 0.f : -m, m == -INFINITY ? 0.f : -m);
                     float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
                     // P over its scores (they are in registers), two keys a column
+                    uint32_t pk[32];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t pk[8];
-#pragma unroll
-                        for (int j = 0; j < 16; j += 2) {
-                            const int at = (i & 1) * 16 + j;
-                            const float2 e = tt_fma2(make_float2(__uint_as_float(x[i >> 1][at]), __uint_as_float(x[i >> 1][at + 1])), c2, minus);
-                            const uint32_t w = pack_bf16(at_exp2(e.x), at_exp2(e.y));
-                            sums[(j >> 1) & 1] = tt_add2(sums[(j >> 1) & 1], make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)));
-                            pk[j >> 1] = w;
-                        }
-                        at_tmem_st8(tS + half * 64 + i * 8, pk);
+                    for (int j = 0; j < 64; j += 2) {
+                        const float2 e = tt_fma2(make_float2(__uint_as_float(x[j >> 5][j & 31]), __uint_as_float(x[j >> 5][(j & 31) + 1])), c2, minus);
+                        const uint32_t w = pack_bf16(at_exp2(e.x), at_exp2(e.y));
+                        sums[(j >> 1) & 1] = tt_add2(sums[(j >> 1) & 1], make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)));
+                        pk[j >> 1] = w;
                     }
+                    at_tmem_st32(tS + half * 64, pk);
                     const float2 sum = tt_add2(sums[0], sums[1]);
                     l += sum.x + sum.y;
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -707,7 +723,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attention_tc_kernel(const 
                 } else {
 #pragma unroll
                     for (int j = 0; j < 32; j += 4)
-                        *reinterpret_cast<float4*>(po + (size_t)pair * D + d + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                        *reinterpret_cast<float4*>(po + ((d + j) / 4 * TT_UNIT + pair) * 4) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -741,7 +757,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) tree_attention_join_kernel(const
     const int mine = (border - 1 - cut.b0) * gridDim.y + blockIdx.y, all = (cut.b1 - cut.b0) * gridDim.y;
     const int from = (int)((long long)elements * mine / all), upto = (int)((long long)elements * (mine + 1) / all);
     for (int e = from + (int)threadIdx.x; e < upto; e += JOIN_THREADS) {
-        const int pair = e / quads, quad = e % quads;
+        const int quad = e / cut.pairs, pair = e - quad * cut.pairs;
         float top = -INFINITY, sum = 0.f;
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int i0 = 0; i0 < parts; i0 += JOIN_AHEAD) {        // (asked for together: a trip to memory for each part was most of this kernel's time)
@@ -753,7 +769,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) tree_attention_join_kernel(const
                 if (i0 + i < parts) {
                     const size_t slot = 2 * (size_t)(cut.b0 + i0 + i) + (i0 + i == 0 ? 1 : 0);
                     its[i] = *reinterpret_cast<const float2*>(ml + (slot * TT_UNIT + pair) * 2);
-                    v[i] = *reinterpret_cast<const float4*>(a.parts + slot * size + (size_t)pair * D + quad * 4);
+                    v[i] = *reinterpret_cast<const float4*>(a.parts + slot * size + (quad * TT_UNIT + pair) * 4);
                 }
             }
 #pragma unroll
@@ -781,6 +797,7 @@ template <int D> static int launch_tree_tc(TtArgs a, int blocks, cudaStream_t st
     CUtensorMap map;
     if (at_make_map(&map, a.pages, D, (cuuint64_t)a.num_pages * 2 * a.G * a.page_size, a.page_size < TT_KEYS ? a.page_size : TT_KEYS)) return ZAI_BAD_SIZE;
     a.dual_cost = D == 128 ? 1 : 2;
+    a.unit_extra = TT_EXTRA;
     static unsigned long long done = 0;
     if (zai_first_on_device(&done)) cudaFuncSetAttribute(tree_attention_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape::SMEM);
     const int code = launch_pdl(tree_attention_tc_kernel<D>, dim3(blocks), dim3(TT_THREADS), Shape::SMEM, stream, map, a);
@@ -812,6 +829,6 @@ ZAI_API int zai_tree_attention_tc(void* out, const void* q, long long q_stride, 
     while ((1 << shift) < page_size) ++shift;
     const long long reach = (long long)table_width * page_size;
     const TtArgs a = {(bf16*)out, (const bf16*)q, (const bf16*)k, (const bf16*)v, (const bf16*)pages, q_stride, k_stride, v_stride, table, cu, ctx,
-                      (const unsigned*)mask, table_width, words, S, N, page_size, shift, num_pages, H, G, H / G, 1, reach > 0x3fffffffll ? 0x3fffffff : (int)reach, scale, parts, status};
+                      (const unsigned*)mask, table_width, words, S, N, page_size, shift, num_pages, H, G, H / G, 1, 0, reach > 0x3fffffffll ? 0x3fffffff : (int)reach, scale, parts, status};
     return D == 64 ? launch_tree_tc<64>(a, blocks, stream) : launch_tree_tc<128>(a, blocks, stream);
 }
