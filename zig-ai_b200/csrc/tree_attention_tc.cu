@@ -1,36 +1,42 @@
 // Attention of trees of drafted tokens on the 5th-generation tensor cores: the same sums as csrc/tree_attention.cu (which says what a row
 // sees), bfloat16 heads of 64 and 128, no window.  Per unit, which is up to 256 (row, query head) pairs of one request and key/value head, and
-// half a tile of 128 keys
+// tile of 64 keys
 //
 //     S = Q K^T      tcgen05.mma, M = 128 pairs (TMEM lanes), N = 64 keys, both operands in shared memory
 //     P = exp2(..)   a pair a thread, from TMEM and back into it over its scores, two bfloat16 a column
 //     O += P V       tcgen05.mma, A in TMEM, V as it lies ([key][column], MN-major), N = the head's columns
 //
-// Eight softmax warps are two turns with scores, O, reference and sum of their own, and a warp each that issues their products: while one half
+// Eight softmax warps are two turns with scores, O, reference and sum of their own, and a warp each that issues their products: while one tile
 // is in the softmax, the other's P is multiplied and its buffer gets the scores after next.  A unit of more than 128 pairs has a turn for
 // each half of its pairs, and each tile of keys serves both; a smaller one has its tiles by turns, and the two O are joined at its end.
 //
-// A tile's keys and its values take a slot each of a ring, laid out in the 128-byte swizzle that the products read.  Tiles of cached keys alone
-// come by TMA, page by page; a unit's last two, which end inside a page or hold the drafted rows, by cp.async from four warps (rows at
-// any 16-byte stride, zeros for keys that are not there).  Nothing is waited for there but a free slot: copies arrive at their barrier by
-// themselves.
+// A tile's keys and its values take a slot each of two rings, laid out in the 128-byte swizzle that the products read.  Tiles of cached keys alone
+// come by TMA, page by page; a unit's last ones, which end inside a page or hold the drafted rows, by cp.async (rows at any 16-byte stride,
+// zeros for keys that are not there).  Nothing is waited for there but a free slot: copies arrive at their barrier by themselves.
 //
 // The work is the list of all units' tiles, cut into equal shares for as many blocks as there are SMs: a block's share may begin and end
 // inside a unit, whose parts then go to memory and are joined by a second kernel.  (Requests of a batch differ in length by a factor of
 // twenty and more; with a block or a cluster a unit the longest decides.)
+//
+// What bounds it, 8 trees of 24-64 rows of 32 heads over 8, heads of 128, behind 4000-30000 positions: 143 us, of which the launches, the list, the
+// first loads and the join some 25; without the softmax 119, without it and most of the products 85.  A tile that serves both turns reads 48 KB of operands for each of
+// them, 1300 cycles of shared memory's 128 bytes a cycle, against 1024 cycles of exponentials.  With heads of 64 (32 trees of 4-24
+// rows behind 300-6000 positions, 63 us) it is the softmax's chain: 64 exponentials a thread and tile are 512 of its 2000 cycles.
 #include "attention_tc_helpers.cuh"
 #include "mma_helpers.cuh"
 
-#define TT_KEYS 128
+#define TT_KEYS 64                      // keys of a tile
 #define TT_TILE 128                     // lanes of a product
 #define TT_UNIT 256                     // pairs of a unit
-#define TT_ROWS 128                     // rows of a tree: one tile of keys
+#define TT_ROWS 128                     // rows of a tree: two tiles of keys
 #define TT_SOFTMAX 8
 #define TT_LOADERS 2                    // (twelve warps leave a thread 168 registers; with four loaders, 128)
-#define TT_SUB (TT_TILE / 32 / TT_LOADERS)      // groups of 32 rows of a tile that a loading warp copies
 #define TT_THREADS (32 * (TT_SOFTMAX + TT_LOADERS + 2))
-#define TT_LEAST 4                      // cost of a share: fewer blocks take part when there is less than this for each
-#define TT_EXTRA 3                      // cost of a unit beside its tiles (its queries, first scores and end)
+#define TT_LEAST 4                      // cost of a share: fewer blocks take part when there is less than this for each (16: 20 instead of 15 us for one tree
+                                        // of 32 rows of 32 heads behind 2000 positions)
+// Cost of a unit beside its tiles: its first scores and its end.  (Blocks with shares of nine short units were the last by a third: none
+// counted 86 us, this 69, when the 32 trees above were measured so.)
+#define TT_EXTRA 6
 #define TT_LOG2E 1.4426950408889634f
 
 struct TtArgs {
@@ -50,10 +56,10 @@ struct TtArgs {
 // ---- the list of tiles.  A request with n rows has units of 256 pairs by key/value head, the last ones of what is left; each unit has a
 // tile for every 128 cached keys and one for the drafted rows.  With heads of 64 a tile that both turns work on costs twice what one of
 // a turn alone does; with heads of 128, where the ring holds two tiles and a turn alone waits for the next, they cost the same.
-struct Request { int first, n, ctx, tiles, row_units, last_cost; };
+struct Request { int first, n, ctx, cached, tiles, row_units, last_cost; };
 __device__ __forceinline__ int unit_cost(const TtArgs& a, int pairs) { return pairs > TT_TILE ? a.dual_cost : 1; }
 __device__ __forceinline__ Request request_of(const TtArgs& a, int s, bool say) {
-    Request r = {0, 0, 0, 0, 0, 0};
+    Request r = {0, 0, 0, 0, 0, 0, 0};
     r.first = a.cu[s];
     r.n = a.cu[s + 1] - r.first;
     r.ctx = max(a.ctx[s], 0);
@@ -74,7 +80,8 @@ __device__ __forceinline__ Request request_of(const TtArgs& a, int s, bool say) 
         if (say) zai_raise(a.status, ZAI_ST_POSITION);
         r.ctx = a.reach;
     }
-    r.tiles = (r.ctx + TT_KEYS - 1) / TT_KEYS + 1;
+    r.cached = (r.ctx + TT_KEYS - 1) / TT_KEYS;
+    r.tiles = r.cached + (r.n + TT_KEYS - 1) / TT_KEYS;
     const int pairs = r.n * a.group;
     r.row_units = (pairs + TT_UNIT - 1) / TT_UNIT;
     r.last_cost = unit_cost(a, pairs - (r.row_units - 1) * TT_UNIT);
@@ -124,7 +131,7 @@ __device__ __forceinline__ int tiles_before(const TtArgs& a, const Place& p, lon
 }
 
 struct Segment {
-    int s, first, n, ctx, pair0, pairs, head, tiles, from, upto;       // key tiles [from, upto) of the unit's `tiles`
+    int s, first, n, ctx, pair0, pairs, head, cached, tiles, from, upto;       // key tiles [from, upto) of the unit's `tiles`, the first of them `cached` ones
     __device__ __forceinline__ bool dual() const { return pairs > TT_TILE; }
     __device__ __forceinline__ bool whole() const { return from == 0 && upto == tiles; }
 };
@@ -169,6 +176,7 @@ struct Walk {
             g.head = p.head;
             g.pair0 = p.row * TT_UNIT;
             g.pairs = min(r.n * a.group - g.pair0, TT_UNIT);
+            g.cached = r.cached;
             g.tiles = r.tiles;
             return true;
         }
@@ -233,6 +241,10 @@ __device__ __forceinline__ void begin_walk(const TtArgs& a, int D, long long* sh
     }
 }
 
+// The two turns' warps of a quarter of the multiprocessor do their exponentials one after the other (64 x 8 cycles of its special-function unit
+// each), while the other waits, loads and compares: 67 instead of 71 us for the 32 trees above, 58 instead of 61 for 8 of 33-64 rows.
+#define TT_SYNC(i) asm volatile("bar.sync %0, 64;" ::"r"(2 + (i)) : "memory")
+#define TT_ARRIVE(i) asm volatile("bar.arrive %0, 64;" ::"r"(2 + (i)) : "memory")
 // two 32-bit numbers in one instruction
 __device__ __forceinline__ float2 tt_fma2(float2 a, float2 b, float2 c) {
     float2 d;
@@ -263,217 +275,216 @@ __device__ __forceinline__ void tt_wait_ld16(uint32_t (&r)[16]) {        // (tie
                    "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
                  :: "memory");
 }
+__device__ __forceinline__ void tt_arrive(uint64_t* bar, int count) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(at_smem(bar)), "r"(count) : "memory");
+}
 // An arrival of this thread's at a barrier when its copies so far have landed
 __device__ __forceinline__ void tt_arrive_landed(uint64_t* bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(at_smem(bar)) : "memory");
 }
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// (a loader's waits are long ones: it naps between its tries, whose instructions the softmax warps would miss)
-__device__ __forceinline__ bool tt_wait_warp(uint64_t* bar, uint32_t parity, volatile int* failed) {
-    return __all_sync(0xffffffffu, at_mbar_wait<AT_NAP_NS>(bar, parity, failed));
-}
+// Where a segment's queries lie: `use` counts the halves (of 128 pairs) taken so far, one by a segment of one turn's pairs, two by another;
+// both turns' product warps wait for all of them, and say of the other's half at once that they are done with it.
+template <int QS> struct Queries {
+    static __device__ __forceinline__ int slot(int use) { return use % QS; }
+    static __device__ __forceinline__ uint32_t round(int use) { return (use / QS) & 1; }
+};
 // What the loaders and the other warps share.
 struct Pipe {
     unsigned char *q, *ring;
     uint64_t *full, *empty, *q_full, *q_empty;
-    volatile int *odd, *failed;         // odd [4] by segment: its number (8 bits) + 1 if a drafted value is not finite
+    volatile int *odd, *failed;         // odd [16] by segment: its number (8 bits) + 1 if a drafted value is not finite
 };
 
-// Where a tile's keys and values lie in the ring, `t` counting all tiles of the block's share, and the round of their slots' barriers.  Keys and
-// values have slots of their own, so that a slot's last tenant was waited for by the same warp that waits for the next: a barrier's parity
-// cannot tell "two phases behind" from "done".  (With two turns' warps that wait for their own tiles alone, KS and VS are even.)
-template <int KS, int VS> struct Ring {
-    static constexpr int SLOTS = KS + VS;
-    static __device__ __forceinline__ int k_slot(int t) { return t % KS; }
-    static __device__ __forceinline__ int v_slot(int t) { return KS + t % VS; }
-    static __device__ __forceinline__ uint32_t k_round(int t) { return (t / KS) & 1; }
-    static __device__ __forceinline__ uint32_t v_round(int t) { return (t / VS) & 1; }
-};
-
-// The loading warps.  D: a head's columns; KS, VS: slots of the ring.
-template <int D, int KS, int VS>
-__device__ __forceinline__ void load_units(const TtArgs& a, const CUtensorMap* pages_map, Walk walk, const Pipe& pipe, int lw) {
-    constexpr int BLOCK = TT_TILE * 128, SLOT = D / 64 * BLOCK, CHUNKS = D / 8;
-    const int lane = threadIdx.x & 31, group = a.group;
-    unsigned char *sQ = pipe.q, *ring = pipe.ring;
-    uint64_t *full = pipe.full, *empty = pipe.empty, *q_full = pipe.q_full, *q_empty = pipe.q_empty;
-    volatile int *odd = pipe.odd, *failed = pipe.failed;
-    Segment g;
-    using R = Ring<KS, VS>;
-    int count = 0, seg = 0;                                 // tiles begun
-    bool ok = true;
-    auto copy_rows = [&](unsigned char* dst, const bf16* mine, int rows) {        // 32 rows of D values, the 32 rows-th of the tile, a row's start in each lane
-#pragma unroll
-        for (int e = 0; e < CHUNKS; ++e) {
-            const int f = e * 32 + lane, r = f / CHUNKS, c = f % CHUNKS, row = rows * 32 + r;
-            const bf16* p = (const bf16*)__shfl_sync(0xffffffffu, (unsigned long long)mine, r);
-            cp_async16(dst + (c >> 3) * BLOCK + row * 128 + (((c & 7) ^ (row & 7)) << 4), p ? p + c * 8 : a.pages, p != nullptr);
+// Where a tile's keys and values lie in the ring, `t` counting all tiles of the block's share, and the round of their slots' barriers.  A barrier's
+// parity cannot tell "two phases behind" from "done", so whoever waits for one of a barrier's phases waits for all of them, in their order, and none
+// ends before all have seen the one before: a turn's product warp waits for the other turn's tiles too, and says so to their slots' barriers.
+template <int SIZE> struct Turning {
+    int at = 0, slot = 0;               // tiles passed; the next one's slot
+    uint32_t round = 0;                 // ... and the round of its barriers, 0 and 1 by turns
+    __device__ __forceinline__ void step() {
+        ++at;
+        if (++slot == SIZE) {
+            slot = 0;
+            round ^= 1;
         }
-    };
+    }
+};
+
+// 32 rows of D values, the 32 rows-th of their block (64 columns every `block` bytes), by a warp with a row's start in each lane; zeros for none
+template <int D> __device__ __forceinline__ void copy_rows(const TtArgs& a, unsigned char* dst, const bf16* mine, int rows, int block) {
+    constexpr int CHUNKS = D / 8;
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int e = 0; e < CHUNKS; ++e) {
+        const int f = e * 32 + lane, r = f / CHUNKS, c = f % CHUNKS, row = rows * 32 + r;
+        const bf16* p = (const bf16*)__shfl_sync(0xffffffffu, (unsigned long long)mine, r);
+        cp_async16(dst + (c >> 3) * block + row * 128 + (((c & 7) ^ (row & 7)) << 4), p ? p + c * 8 : a.pages, p != nullptr);
+    }
+}
+
+// The two loading warps: one brings keys, the other queries and values (a tile's values are used two tiles of its turn after its keys: when one
+// warp brought both, values held their slots for that long beforehand and keys came late, 112 instead of 89 us for 32 trees of 4-24 rows
+// behind 300-6000 positions with heads of 128).  A warp's chain of instructions for a tile is some 700 cycles, so each does its own walk and nothing else.
+template <int D, typename Shape, bool VALUES>
+__device__ __forceinline__ void load_tiles(const TtArgs& a, const CUtensorMap* pages_map, Walk walk, const Pipe& pipe) {
+    using Q = Queries<Shape::QS>;
+    constexpr int BLOCK = Shape::BLOCK, SLOT = Shape::SLOT, SIZE = VALUES ? Shape::VS : Shape::KS, CHUNKS = D / 8;
+    const int lane = threadIdx.x & 31, group = a.group;
+    unsigned char* ring = pipe.ring + (VALUES ? Shape::KS * SLOT : 0);
+    uint64_t *full = pipe.full + (VALUES ? Shape::KS : 0), *empty = pipe.empty + (VALUES ? Shape::KS : 0);
+    volatile int* failed = pipe.failed;
+    const int box = min(a.page_size, TT_KEYS), boxes = TT_KEYS / box;
+    Segment g;
+    int count = 0, seg = 0, use = 0;                        // tiles begun, segments, halves of queries
+    bool ok = true;
     while (ok && walk.next(a, g)) {
+        // the queries, as many segments ahead as there is room for, so that a unit's first scores need not wait for them
+        for (int h = 0; VALUES && h < (g.dual() ? 2 : 1) && ok; ++h, ++use) {
+            const int slot = Q::slot(use);
+            ok = at_mbar_wait_warp(&pipe.q_empty[slot], Q::round(use) ^ 1, failed);
+            if (!ok) break;
+#pragma unroll
+            for (int rows = 0; rows < TT_TILE / 32; ++rows) {
+                const int r = h * TT_TILE + rows * 32 + lane, p = g.pair0 + r;
+                copy_rows<D>(a, pipe.q + slot * Shape::QSLOT,
+                             r < g.pairs ? a.q + (long long)(g.first + p / group) * a.q_stride + (g.head * group + p % group) * D : nullptr, rows, Shape::QBLOCK);
+            }
+            tt_arrive_landed(&pipe.q_full[slot]);
+        }
         const int* table = a.table + (size_t)g.s * a.table_width;
-        // The tiles that hold 128 cached keys: a lane's page of the tile is asked for a tile ahead.  The others: where this lane's key lies.
-        const int whole = g.ctx / TT_KEYS, box = min(a.page_size, TT_KEYS), boxes = TT_KEYS / box;
-        auto checked = [&](int page, int idx) {
+        const int whole = g.ctx / TT_KEYS, used = (g.ctx + a.page_size - 1) >> a.page_shift;
+        // entries of the block table, 32 at a time, one a lane; the next 32 are asked for when these come to use
+        auto ask = [&](int first) { return first + lane < used && first + lane < a.table_width ? table[first + lane] : -1; };
+        int entries0 = ((g.from * TT_KEYS) >> a.page_shift) & ~31, entries = ask(entries0), next = ask(entries0 + 32);
+        auto entry = [&](int idx, bool needed) {            // the page at a lane's own idx of these
+            const int page = __shfl_sync(0xffffffffu, entries, idx & 31);
             if ((unsigned)page < (unsigned)a.num_pages) return page;
-            zai_raise(a.status, idx < a.table_width ? ZAI_ST_PAGE : ZAI_ST_POSITION);
+            if (needed) zai_raise(a.status, ZAI_ST_PAGE);
             return 0;
         };
-        auto ask = [&](int tile) {
-            const int idx = (tile * TT_KEYS + lane * box) >> a.page_shift;
-            return tile < whole && tile < g.upto && lane < boxes && idx < a.table_width ? table[idx] : -1;
-        };
-        auto find = [&](int tile, int rows, const bf16*& kp, const bf16*& vp) {
-            const int node = rows * 32 + lane, key = tile * TT_KEYS + node;
-            kp = vp = nullptr;
-            if (tile == g.tiles - 1) {
-                if (node < g.n) {
-                    kp = a.k + (long long)(g.first + node) * a.k_stride + g.head * D;
-                    vp = a.v + (long long)(g.first + node) * a.v_stride + g.head * D;
-                }
-            } else if (key < g.ctx) {
-                const int idx = key >> a.page_shift, page = checked(idx < a.table_width ? table[idx] : -1, idx);
-                kp = a.pages + (((long long)page * 2 * a.G + g.head) * a.page_size + (key & (a.page_size - 1))) * D;
-                vp = kp + (long long)a.G * a.page_size * D;
-            }
-        };
-        // the queries go to where the last unit's lie: its last scores come first, and keys and values need not wait for that
-        bool have_q = false;
-        auto queries = [&](bool wait) {
-            const uint32_t parity = (seg & 1) ^ 1;
-            if (wait) ok = tt_wait_warp(q_empty, parity, failed);
-            else if (!__all_sync(0xffffffffu, at_mbar_test(q_empty, parity))) return;
-            if (!ok) return;
-            for (int h = 0; h < (g.dual() ? 2 : 1); ++h)
-#pragma unroll
-                for (int u = 0; u < TT_SUB; ++u) {
-                    const int r = h * TT_TILE + (lw * TT_SUB + u) * 32 + lane, p = g.pair0 + r;
-                    copy_rows(sQ + h * SLOT, r < g.pairs ? a.q + (long long)(g.first + p / group) * a.q_stride + (g.head * group + p % group) * D : nullptr, lw * TT_SUB + u);
-                }
-            tt_arrive_landed(q_full);
-            have_q = true;
-        };
-        int page = ask(g.from), next = -1;
-        const bf16 *kp[TT_SUB] = {}, *vp[TT_SUB] = {};
-        for (int i = 0; i < 2 * (g.upto - g.from) && ok; count += i & 1, ++i) {
-            const int slot = i & 1 ? R::v_slot(count) : R::k_slot(count), tile = g.from + (i >> 1);
-            const uint32_t parity = (i & 1 ? R::v_round(count) : R::k_round(count)) ^ 1;
-            if (!have_q) queries(i >= 2 * (KS < VS ? KS : VS) - 1);
-            // (a slot that is in use may be one of this unit's own, which its queries free)
-            if (ok && !have_q && !__all_sync(0xffffffffu, at_mbar_test(&empty[slot], parity))) queries(true);
-            if (ok) ok = tt_wait_warp(&empty[slot], parity, failed);
-            if (!ok) break;
+        for (int tile = g.from; tile < g.upto; ++tile, ++count) {
+            const int slot = count % SIZE;
             unsigned char* dst = ring + (size_t)slot * SLOT;
-            if (tile < whole) {
-                if (!(i & 1)) {
-                    page = lane < boxes ? checked(page, (tile * TT_KEYS + lane * box) >> a.page_shift) : 0;
-                    next = ask(tile + 1);
+            if ((tile * TT_KEYS) >> a.page_shift >= entries0 + 32) {
+                entries0 += 32;
+                entries = next;
+                next = ask(entries0 + 32);
+            }
+            if (tile < whole) {                             // a lane a page
+                const int at = tile * TT_KEYS + lane * box, page = entry(at >> a.page_shift, lane < boxes);
+                ok = at_mbar_wait_warp(&empty[slot], (count / SIZE & 1) ^ 1, failed);
+                if (!ok) break;
+                if (lane == 0) {                            // (all of the barrier's 32 arrivals)
+                    at_mbar_expect_tx(&full[slot], SLOT);
+                    tt_arrive(&full[slot], 31);
                 }
-                if (lw == 0) {                              // (the others' arrivals make up the barrier's count)
-                    if (lane == 0) at_mbar_expect_tx(&full[slot], SLOT);
-                    else at_mbar_arrive(&full[slot]);
-                    __syncwarp();
-                    if (lane < boxes) {                     // a lane a page
-                        const int row = ((page * 2 + (i & 1)) * a.G + g.head) * a.page_size + ((tile * TT_KEYS + lane * box) & (a.page_size - 1));
+                __syncwarp();
+                if (lane < boxes) {
+                    const int row = ((page * 2 + (VALUES ? 1 : 0)) * a.G + g.head) * a.page_size + (at & (a.page_size - 1));
 #pragma unroll
-                        for (int c = 0; c < D / 64; ++c)
-                            at_tma_load_2d(dst + c * BLOCK + lane * box * 128, pages_map, c * 64, row, &full[slot]);
-                    }
-                } else at_mbar_arrive(&full[slot]);
-                if (i & 1) page = next;
+                    for (int c = 0; c < D / 64; ++c) at_tma_load_2d(dst + c * BLOCK + lane * box * 128, pages_map, c * 64, row, &full[slot]);
+                }
                 continue;
             }
-            if (!(i & 1)) {
+            // a tile that ends inside a page, or of drafted rows: by cp.async, a row's start in each lane, zeros for what is not there
+            const bool drafted = tile >= g.cached;
+            const bf16* from[2];
+            bool bad = false;
 #pragma unroll
-                for (int u = 0; u < TT_SUB; ++u) {
-                    find(tile, lw * TT_SUB + u, kp[u], vp[u]);
-                    copy_rows(dst, kp[u], lw * TT_SUB + u);
+            for (int u = 0; u < 2; ++u) {
+                const int at = u * 32 + lane;
+                from[u] = nullptr;
+                if (drafted) {
+                    const int node = (tile - g.cached) * TT_KEYS + at;
+                    if (node < g.n) from[u] = (VALUES ? a.v + (long long)(g.first + node) * a.v_stride : a.k + (long long)(g.first + node) * a.k_stride) + g.head * D;
+                } else {
+                    const int key = tile * TT_KEYS + at, page = entry(min(key, g.ctx - 1) >> a.page_shift, key < g.ctx);
+                    if (key < g.ctx) from[u] = a.pages + ((((long long)page * 2 + (VALUES ? 1 : 0)) * a.G + g.head) * a.page_size + (key & (a.page_size - 1))) * D;
                 }
-            } else {
-                bool bad = false;                           // is one of this lane's values, drafted ones, not finite?  (A look at memory: to wait for the
+            }
+            ok = at_mbar_wait_warp(&empty[slot], (count / SIZE & 1) ^ 1, failed);
+            if (!ok) break;
 #pragma unroll
-                for (int u = 0; u < TT_SUB; ++u) {          // copies would hold up the next unit's)
-                    copy_rows(dst, vp[u], lw * TT_SUB + u);
-                    if (tile != g.tiles - 1 || !vp[u]) continue;
+            for (int u = 0; u < 2; ++u) copy_rows<D>(a, dst, from[u], u, BLOCK);
+            if (VALUES && drafted)                          // is one of the drafted values not finite?  (A look of its own at memory: to wait for the copies
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {               // would hold up the next unit's)
+                    if (!from[u]) continue;
                     uint4 x[CHUNKS];
 #pragma unroll
-                    for (int c = 0; c < CHUNKS; ++c) x[c] = *reinterpret_cast<const uint4*>(vp[u] + c * 8);
+                    for (int c = 0; c < CHUNKS; ++c) x[c] = *reinterpret_cast<const uint4*>(from[u] + c * 8);
 #pragma unroll
                     for (int c = 0; c < CHUNKS; ++c) bad |= at_not_finite(x[c]);
                 }
-                if (__any_sync(0xffffffffu, bad)) {         // zeros in their place (what a row sees is put right at its end)
-                    cp_async_wait_all();
-                    bool mine = false;
-                    __syncwarp();
-                    for (int e = 0; e < CHUNKS * TT_SUB; ++e) {
-                        const int f = e * 32 + lane, key = lw * TT_SUB * 32 + f / CHUNKS, c = f % CHUNKS;
-                        unsigned char* at = dst + (c >> 3) * BLOCK + key * 128 + (((c & 7) ^ (key & 7)) << 4);
-                        if (at_not_finite(*reinterpret_cast<const uint4*>(at))) {
-                            mine = true;
-                            unsigned short* v = reinterpret_cast<unsigned short*>(at);
-                            for (int x = 0; x < 8; ++x)
-                                if ((v[x] & 0x7f80) == 0x7f80) v[x] = 0;
-                        }
+            if (VALUES && __any_sync(0xffffffffu, bad)) {   // zeros in their place (what a row sees is put right at its end)
+                cp_async_wait_all();
+                for (int e = 0; e < 2 * CHUNKS; ++e) {
+                    const int f = e * 32 + lane, key = f / CHUNKS, c = f % CHUNKS;
+                    unsigned char* at = dst + (c >> 3) * BLOCK + key * 128 + (((c & 7) ^ (key & 7)) << 4);
+                    if (at_not_finite(*reinterpret_cast<const uint4*>(at))) {
+                        pipe.odd[seg & 15] = (seg & 0xff) + 1;
+                        unsigned short* v = reinterpret_cast<unsigned short*>(at);
+                        for (int u = 0; u < 8; ++u)
+                            if ((v[u] & 0x7f80) == 0x7f80) v[u] = 0;
                     }
-                    if (mine) odd[seg & 3] = (seg & 0xff) + 1;
-                    at_proxy_fence();
-                    at_mbar_arrive(&full[slot]);
-                    continue;
                 }
-            }
-            tt_arrive_landed(&full[slot]);
+                at_proxy_fence();
+                at_mbar_arrive(&full[slot]);
+            } else tt_arrive_landed(&full[slot]);
         }
-        if (ok && !have_q) queries(true);
         ++seg;
     }
     cp_async_wait_all();
-    if (!ok && lw == 0)                                     // a wait ran out: the tiles still on their way are waited for, with a limit, before the block ends
-        for (int t = max(count - (KS > VS ? KS : VS), 0); t <= count; ++t)
-            for (int spin = 0; spin < AT_SPIN_LIMIT && !(at_mbar_test(&full[R::k_slot(t)], R::k_round(t)) && at_mbar_test(&full[R::v_slot(t)], R::v_round(t))); ++spin) {}
+    if (!ok && lane < SIZE)                                 // a wait ran out: the copies still on their way are waited for, with a limit, before the block ends
+        for (int t = max(count - SIZE, 0); t < count; ++t)
+            if (t % SIZE == lane)
+                for (int spin = 0; spin < AT_SPIN_LIMIT && !at_mbar_test(&full[lane], (t / SIZE) & 1); ++spin) {}
 }
 
 template <int D> struct TtShape {
-    static constexpr int BLOCK = TT_TILE * 128;                 // 64 columns of 128 rows, a swizzled row of 128 bytes each
-    static constexpr int SLOT = D / 64 * BLOCK;                 // a tile's keys or values, or 128 pairs of Q
-    static constexpr int KS = D == 128 ? 2 : 6, VS = KS, SLOTS = KS + VS;
-    static constexpr int COLS = 256 + 2 * D;                    // TMEM: two score buffers, two O
-    static constexpr int ALLOC = 512;
-    static constexpr size_t TILES = (size_t)(2 + SLOTS) * SLOT;
-    static constexpr size_t SMEM = TILES + sizeof(float) * 4 * TT_TILE + 8 * (2 * SLOTS + 14 + 3) + 32;
+    static constexpr int BLOCK = TT_KEYS * 128;                 // 64 columns of a tile's keys or values, a swizzled row of 128 bytes each
+    static constexpr int SLOT = D / 64 * BLOCK;
+    static constexpr int QBLOCK = TT_TILE * 128, QSLOT = D / 64 * QBLOCK;     // ... of 128 pairs' queries
+    static constexpr int KS = 20 / (D / 64) / 2, VS = KS, SLOTS = KS + VS, QS = D == 128 ? 2 : 4;
+    static_assert(KS >= 4 && VS >= 4, "two tiles are brought at once, and scores run two of a turn's tiles ahead of their products");
+    static constexpr int ALLOC = 512;                           // TMEM: 256 columns for four score buffers, two O
+    static constexpr size_t TILES = (size_t)QS * QSLOT + (size_t)SLOTS * SLOT;
+    static constexpr size_t SMEM = TILES + sizeof(float) * 4 * TT_TILE + 8 * (2 * SLOTS + 10 + 2 * QS + 2 + 3) + 4 * 20;
 };
 
 template <int D>
 __global__ void __launch_bounds__(TT_THREADS, 1) tree_attention_tc_kernel(const __grid_constant__ CUtensorMap pages_map, const TtArgs a) {
     using Shape = TtShape<D>;
-    using R = Ring<Shape::KS, Shape::VS>;
-    constexpr int SLOT = Shape::SLOT, SLOTS = Shape::SLOTS;
+    using Q = Queries<Shape::QS>;
+    constexpr int SLOT = Shape::SLOT, SLOTS = Shape::SLOTS, QS = Shape::QS;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    unsigned char* sQ = smem_raw;                               // [2][SLOT]
-    unsigned char* ring = smem_raw + 2 * SLOT;                  // [SLOTS][SLOT]
+    unsigned char* sQ = smem_raw;                               // [QS][QSLOT]
+    unsigned char* ring = smem_raw + QS * Shape::QSLOT;                 // [SLOTS][SLOT]
     float* exch = reinterpret_cast<float*>(smem_raw + Shape::TILES);   // [2][2][128]: maxima, then sums, by turn
     uint64_t* full = reinterpret_cast<uint64_t*>(exch + 4 * TT_TILE);  // [SLOTS]
     uint64_t* empty = full + SLOTS;                             // [SLOTS]
-    uint64_t* s_ready = empty + SLOTS;                          // [2][2] a turn's scores, of the first and second half of a tile's keys
+    uint64_t* s_ready = empty + SLOTS;                          // [2][2] a turn's scores, of its even and odd tiles
     uint64_t* p_ready = s_ready + 4;                            // [2][2] ... P
     uint64_t* o_done = p_ready + 4;                             // [2] a turn's last product is in O
-    uint64_t* q_full = o_done + 2;                              // a segment's queries
-    uint64_t* q_empty = q_full + 1;                             // ... its last scores are made
-    uint64_t* o_full = q_empty + 1;                             // a segment's last products are in O
+    uint64_t* q_full = o_done + 2;                              // [QS] queries of 128 pairs
+    uint64_t* q_empty = q_full + QS;                            // [QS] ... their last scores are made
+    uint64_t* o_full = q_empty + QS;                            // a segment's last products are in O
     uint64_t* o_empty = o_full + 1;                             // ... and have been read
     long long* share = reinterpret_cast<long long*>(o_empty + 1);      // the block's walk: pos, end, base
     int* words = reinterpret_cast<int*>(share + 3);
     uint32_t& tmem_holder = reinterpret_cast<uint32_t*>(words)[0];
     int& failed_flag = words[1];
     int& s_first = words[2];
-    volatile int* odd = words + 4;                              // [4] by segment: its number (8 bits) + 1 if a drafted value is not finite
+    volatile int* odd = words + 4;                              // [16] by segment: its number (8 bits) + 1 if a drafted value is not finite
     volatile int* failed = &failed_flag;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = a.group;
 
     if (tid == 0) {
         failed_flag = (at_smem(sQ) & 1023u) ? 1 : 0;            // the swizzled tiles need 1024-byte alignment
         for (int i = 0; i < SLOTS; ++i) {
-            at_mbar_init(&full[i], 32 * TT_LOADERS);
+            at_mbar_init(&full[i], 32);
             at_mbar_init(&empty[i], 2);
         }
         for (int i = 0; i < 4; ++i) {
@@ -481,11 +492,13 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attention_tc_kernel(const 
             at_mbar_init(&p_ready[i], 4);
             if (i < 2) at_mbar_init(&o_done[i], 1);
         }
-        at_mbar_init(q_full, 32 * TT_LOADERS);
-        at_mbar_init(q_empty, 2);
+        for (int i = 0; i < QS; ++i) {
+            at_mbar_init(&q_full[i], 32);
+            at_mbar_init(&q_empty[i], 2);
+        }
         at_mbar_init(o_full, 2);
         at_mbar_init(o_empty, TT_SOFTMAX);
-        for (int i = 0; i < 4; ++i) odd[i] = 0;
+        for (int i = 0; i < 16; ++i) odd[i] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == TT_SOFTMAX + TT_LOADERS) {
@@ -505,75 +518,99 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attention_tc_kernel(const 
     if (failed_flag) {
         // (nothing to wait for)
     } else if (warp >= TT_SOFTMAX && warp < TT_SOFTMAX + TT_LOADERS) {
-        load_units<D, Shape::KS, Shape::VS>(a, &pages_map, walk, Pipe{sQ, ring, full, empty, q_full, q_empty, odd, failed}, warp - TT_SOFTMAX);
+        const Pipe pipe = {sQ, ring, full, empty, q_full, q_empty, odd, failed};
+        if (warp == TT_SOFTMAX) load_tiles<D, Shape, false>(a, &pages_map, walk, pipe);
+        else load_tiles<D, Shape, true>(a, &pages_map, walk, pipe);
     } else if (warp >= TT_SOFTMAX + TT_LOADERS) {
         if (zai_elect()) {
-            // ---- products, a warp a turn, half a tile's keys at a time: while one half is in the softmax, the other's P is multiplied and its buffer
-            // gets the scores after next.  Instruction descriptors: D 32-bit, A and B bfloat16, M = 128; the scores have both operands K-major, O
-            // has P in TMEM and V MN-major, blocks of 64 columns.
-            constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TT_KEYS / 2 >> 3) << 17) | ((uint32_t)(TT_TILE >> 4) << 24);
+            // ---- products, a warp a turn: while one tile is in the softmax, the other's P is multiplied and its buffer gets the scores after next.
+            // Instruction descriptors: D 32-bit, A and B bfloat16, M = 128; the scores have both operands K-major, O has P in TMEM and V MN-major,
+            // blocks of 64 columns.
+            constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TT_KEYS >> 3) << 17) | ((uint32_t)(TT_TILE >> 4) << 24);
             constexpr uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(TT_TILE >> 4) << 24);
             constexpr uint64_t V_BLOCKS = (uint64_t)(Shape::BLOCK / 16 - 1) << 16;     // from 64 columns of V to the next (at_desc's field holds 1)
             const int turn = warp - TT_SOFTMAX - TT_LOADERS;
             const uint32_t tS = tmem + turn * 128, tO = tmem + 256 + turn * D;
-            int count = 0, seg = 0, made = 0;                   // tiles before the segment; the turn's tiles so far
+            const uint64_t dQ = at_desc(at_smem(sQ)), dR = at_desc(at_smem(ring));     // (an address is a field of 14 bits, in 16 bytes: offsets are added)
+            int count = 0, seg = 0, made = 0, use = 0;          // tiles before the segment; the turn's tiles before it; halves of queries
+            Turning<Shape::KS> keys;                            // tiles whose keys, and whose values, have been waited for
+            Turning<Shape::VS> values;
             bool ok = true;
             while (ok && walk.next(a, g)) {
                 const bool dual = g.dual();
-                const int tiles = g.upto - g.from, t0 = dual ? 0 : turn, step = dual ? 1 : 2, jobs = t0 < tiles ? 2 * ((tiles - t0 + step - 1) / step) : 0;
-                const uint32_t aQ = at_smem(sQ) + (dual ? turn * SLOT : 0);
-                // what both turns have to say before a slot, the queries or O count as done, a turn that has no part in it says at once
-                auto scores = [&](int j) {
-                    const int t = t0 + (j >> 1) * step, half = j & 1, slot = R::k_slot(count + t);
-                    if (!half) {
-                        ok = at_mbar_wait(&full[slot], R::k_round(count + t), failed);
-                        if (!ok) return;
-                        at_proxy_fence();                       // (the copies are generic writes, which the products read)
+                const int tiles = g.upto - g.from, t0 = dual ? 0 : turn, step = dual ? 1 : 2, jobs = t0 < tiles ? (tiles - t0 + step - 1) / step : 0;
+                const int q_slot = Q::slot(use + (dual ? turn : 0));
+                const uint64_t q0 = dQ + q_slot * (Shape::QSLOT / 16);
+                // waits for the tiles up to t (or takes note of those that are there); a slot is free when both turns are done with it
+                auto see = [&](auto& ring_at, int base, int t, bool wait) {
+                    while (ring_at.at <= t && ok) {
+                        const int slot = base + ring_at.slot;
+                        if (wait) ok = at_mbar_wait(&full[slot], ring_at.round, failed);
+                        else if (!at_mbar_test(&full[slot], ring_at.round)) return;
+                        if (!dual && ((ring_at.at - count) & 1) != turn) at_mbar_arrive(&empty[slot]);
+                        ring_at.step();
                     }
-                    const uint32_t aK = at_smem(ring + (size_t)slot * SLOT) + half * (TT_KEYS / 2 * 128);
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                };
+                // (the last tile seen is the one that was asked for)
+                auto slot_seen = [](const auto& ring_at, int size) { return ring_at.slot ? ring_at.slot - 1 : size - 1; };
+                auto scores = [&](int j, int slot) {
+                    const int buffer = (made + j) & 1;
+                    const uint64_t k0 = dR + slot * (SLOT / 16);
 #pragma unroll
                     for (int c = 0; c < D / 16; ++c)
-                        at_umma(tS + half * 64, at_desc(aQ + (c >> 2) * Shape::BLOCK + (c & 3) * 32), at_desc(aK + (c >> 2) * Shape::BLOCK + (c & 3) * 32), idesc_s,
+                        at_umma(tS + buffer * 64, q0 + ((c >> 2) * Shape::QBLOCK + (c & 3) * 32) / 16, k0 + ((c >> 2) * Shape::BLOCK + (c & 3) * 32) / 16, idesc_s,
                                 c > 0 ? 1u : 0u);
-                    at_commit(&s_ready[turn * 2 + half]);
-                    if (half) {
-                        at_commit(&empty[slot]);
-                        if (!dual) at_mbar_arrive(&empty[slot]);
-                    }
-                    if (j == jobs - 1) at_commit(q_empty);
+                    at_commit(&s_ready[turn * 2 + buffer]);
+                    at_commit(&empty[slot]);
+                    if (j == jobs - 1) at_commit(&q_empty[q_slot]);
                 };
-                auto product = [&](int j) {
-                    const int t = t0 + (j >> 1) * step, half = j & 1, slot = R::v_slot(count + t);
-                    if (!half) ok = at_mbar_wait(&full[slot], R::v_round(count + t), failed);
-                    if (ok) ok = at_mbar_wait(&p_ready[turn * 2 + half], made & 1, failed);
-                    if (!ok) return;
-                    if (!half) at_proxy_fence();
-                    const uint32_t aV = at_smem(ring + (size_t)slot * SLOT) + half * (TT_KEYS / 2 * 128);
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-                    for (int kk = 0; kk < TT_KEYS / 32; ++kk)   // 16 keys a step: eight columns of P, two groups of 8 keys of V
-                        at_umma_ts(tO, tS + half * 64 + kk * 8, at_desc(aV + kk * 2048) + V_BLOCKS, idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
-                    at_commit(&o_done[turn]);
-                    if (half) {
-                        ++made;
-                        at_commit(&empty[slot]);
-                        if (!dual) at_mbar_arrive(&empty[slot]);
-                    }
-                };
-                ok = at_mbar_wait(q_full, seg & 1, failed);
-                if (jobs == 0) at_mbar_arrive(q_empty);
+                for (int h = 0; h < (dual ? 2 : 1) && ok; ++h) {
+                    ok = at_mbar_wait(&q_full[Q::slot(use + h)], Q::round(use + h), failed);
+                    if (dual && h != turn) at_mbar_arrive(&q_empty[Q::slot(use + h)]);
+                }
+                if (jobs == 0) at_mbar_arrive(&q_empty[q_slot]);
                 else {
-                    if (ok) scores(0);
-                    if (ok) scores(1);
+                    for (int j = 0; j < min(jobs, 2) && ok; ++j) {
+                        see(keys, 0, count + t0 + j * step, true);
+                        if (!ok) break;
+                        at_proxy_fence();                       // (copies by cp.async are generic writes, which the products read)
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        scores(j, slot_seen(keys, Shape::KS));
+                    }
                 }
                 if (ok && seg > 0) ok = at_mbar_wait(o_empty, (seg - 1) & 1, failed);
                 for (int j = 0; j < jobs && ok; ++j) {
-                    product(j);
-                    if (ok && j + 2 < jobs) scores(j + 2);
+                    // (P last: what follows it is the softmax's wait for its next scores)
+                    const int buffer = (made + j) & 1, after = count + t0 + (j + 2) * step;
+                    see(values, Shape::KS, count + t0 + j * step, true);
+                    const int slot = Shape::KS + slot_seen(values, Shape::VS);
+                    if (j + 2 < jobs) see(keys, 0, after, false);
+                    at_proxy_fence();
+                    if (ok) ok = at_mbar_wait(&p_ready[turn * 2 + buffer], ((made + j) >> 1) & 1, failed);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint64_t v0 = dR + V_BLOCKS + slot * (SLOT / 16);
+#pragma unroll
+                    for (int kk = 0; kk < TT_KEYS / 16; ++kk)   // 16 keys a step: eight columns of P, two groups of 8 keys of V
+                        at_umma_ts(tO, tS + buffer * 64 + kk * 8, v0 + kk * (2048 / 16), idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
+                    at_commit(&o_done[turn]);
+                    at_commit(&empty[slot]);
+                    if (j + 2 < jobs) {
+                        if (keys.at <= after) {
+                            see(keys, 0, after, true);
+                            if (!ok) break;
+                            at_proxy_fence();
+                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        }
+                        scores(j + 2, slot_seen(keys, Shape::KS));
+                    }
                 }
                 if (ok) at_commit(o_full);
+                see(keys, 0, count + tiles - 1, true);
+                see(values, Shape::KS, count + tiles - 1, true);
+                made += jobs;
                 count += tiles;
+                use += dual ? 2 : 1;
                 ++seg;
             }
             if (!ok) *failed = 1;
@@ -584,87 +621,102 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attention_tc_kernel(const 
         const int turn = warp >> 2, qd = warp & 3, row = qd * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(qd * 32) << 16), tS = lanes + turn * 128, tO = lanes + 256 + turn * D;
         const float c = a.scale * TT_LOG2E;
-        int seg = 0, taken = 0, jobs = 0;                       // the turn's tiles so far, and their halves
+        int seg = 0, taken = 0;                                 // segments, the turn's tiles so far
         bool ok = true;                                         // (a warp that gives up still meets the others at their barriers)
         while (walk.next(a, g)) {
             const bool dual = g.dual();
             const int pair = dual ? turn * TT_TILE + row : row, p = g.pair0 + pair, node = p / group;
             const bool valid = pair < g.pairs, idle = __all_sync(0xffffffffu, !valid);
             float m = -INFINITY, l = 0.f;
-            int done = 0;
-            for (int tile = g.from + (dual ? 0 : turn); tile < g.upto && ok; tile += dual ? 1 : 2, ++taken)
-                for (int half = 0; half < 2; ++half, ++done) {
-                    ok = at_mbar_wait_warp(&s_ready[turn * 2 + half], taken & 1, failed);
-                    if (!ok) break;
-                    if (idle) {                                 // (its lanes of P and O are nobody's)
-                        ++jobs;
-                        if (lane == 0) at_mbar_arrive(&p_ready[turn * 2 + half]);
-                        continue;
-                    }
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    uint32_t x[2][32];
-                    at_tmem_ld32_nowait(tS + half * 64, x[0]);
-                    at_tmem_ld32_nowait(tS + half * 64 + 32, x[1]);
-                    at_tmem_wait_ld(x[0]);
-                    at_tmem_wait_ld(x[1]);
-                    const bool nodes = tile == g.tiles - 1;
-                    if (nodes || (tile + 1) * TT_KEYS > g.ctx)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {           // which of keys 32 i .. of the half this pair sees
-                            const int word = half * 2 + i, left = (nodes ? g.n : g.ctx - tile * TT_KEYS) - 32 * word;
-                            uint32_t bits = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1;
-                            if (nodes) bits &= valid && word < a.words ? a.mask[(size_t)(g.first + node) * a.words + word] : 0u;
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (!(bits >> j & 1)) x[i][j] = __float_as_uint(-INFINITY);
-                        }
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};         // four chains, not one of 64 links
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int j = 0; j < 32; j += 2)
-                                                        mx[(j >> 1) & 3] = tt_max3(mx[(j >> 1) & 3], __uint_as_float(x[i][j]), __uint_as_float(x[i][j + 1]));
-                    // The reference is the first half's maximum, and moves when a later one exceeds it by 2^8: a weight keeps its 8 bits whatever the
-                    // reference is, and the sum is that of the rounded weights, so what one key dominates stays exact.
-                    const float most = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
-                    const float top = done == 0 || m == -INFINITY ? most : most > m + 8.f ? most : m;
-                    if (done > 0 && __any_sync(0xffffffffu, top != m)) {
-                        // O with the turn's last product in it (those before it came ahead of these scores)
-                        const float keep = m == -INFINITY ? 0.f : at_exp2(m - top);
-                        l *= keep;
-                        ok = at_mbar_wait_warp(&o_done[turn], (jobs + 1) & 1, failed);
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll 1
-                        for (int d = 0; d < D; d += 16) {
-                            uint32_t y[16];
-                            tt_ld16_nowait(tO + d, y);
-                            tt_wait_ld16(y);
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) y[j] = __float_as_uint(__uint_as_float(y[j]) * keep);
-                            at_tmem_st16(tO + d, y);
-                        }
-                    }
-                    m = top;
-                    ++jobs;
-                    const float2 c2 = make_float2(c, c), minus = make_float2(m == -INFINITY ? 0.f : -m, m == -INFINITY ? 0.f : -m);
-                    float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-                    // P over its scores (they are in registers), two keys a column
-                    uint32_t pk[32];
-#pragma unroll
-                    for (int j = 0; j < 64; j += 2) {
-                        const float2 e = tt_fma2(make_float2(__uint_as_float(x[j >> 5][j & 31]), __uint_as_float(x[j >> 5][(j & 31) + 1])), c2, minus);
-                        const uint32_t w = pack_bf16(at_exp2(e.x), at_exp2(e.y));
-                        sums[(j >> 1) & 1] = tt_add2(sums[(j >> 1) & 1], make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)));
-                        pk[j >> 1] = w;
-                    }
-                    at_tmem_st32(tS + half * 64, pk);
-                    const float2 sum = tt_add2(sums[0], sums[1]);
-                    l += sum.x + sum.y;
-                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) at_mbar_arrive(&p_ready[turn * 2 + half]);
+            bool begun = false;
+            // how many tiles the two warps take turns at: as many for one as for the other
+            const bool paired = !idle && (!dual || TT_TILE + qd * 32 < g.pairs);
+            int left = paired ? (dual ? g.upto - g.from : (g.upto - g.from + 1) >> 1) : 0;
+            if (paired && turn == 1) TT_ARRIVE(qd);
+            for (int tile = g.from + (dual ? 0 : turn); tile < g.upto && ok; tile += dual ? 1 : 2, ++taken) {
+                const int buffer = taken & 1;
+                const uint32_t tB = tS + buffer * 64;
+                ok = at_mbar_wait_warp(&s_ready[turn * 2 + buffer], (taken >> 1) & 1, failed);
+                if (!ok) break;
+                if (idle) {                                     // (its lanes of P and O are nobody's)
+                    if (lane == 0) at_mbar_arrive(&p_ready[turn * 2 + buffer]);
+                    continue;
                 }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                uint32_t x[2][32];
+                at_tmem_ld32_nowait(tB, x[0]);
+                at_tmem_ld32_nowait(tB + 32, x[1]);
+                at_tmem_wait_ld(x[0]);
+                at_tmem_wait_ld(x[1]);
+                const bool nodes = tile >= g.cached;
+                if (nodes || (tile + 1) * TT_KEYS > g.ctx)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {               // which of keys 32 i .. of the tile this pair sees
+                        const int word = (tile - g.cached) * 2 + i, there = nodes ? g.n - 32 * word : g.ctx - tile * TT_KEYS - 32 * i;
+                        uint32_t bits = there >= 32 ? 0xffffffffu : there <= 0 ? 0u : (1u << there) - 1;
+                        if (nodes) bits &= valid && word < a.words ? a.mask[(size_t)(g.first + node) * a.words + word] : 0u;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (!(bits >> j & 1)) x[i][j] = __float_as_uint(-INFINITY);
+                    }
+                float mx[8] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY};         // eight chains, not one of 64 links
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2)
+                        mx[(j >> 1) & 7] = tt_max3(mx[(j >> 1) & 7], __uint_as_float(x[i][j]), __uint_as_float(x[i][j + 1]));
+                // The reference is the first tile's maximum, and moves when a later one exceeds it by 2^8: a weight keeps its 8 bits whatever the
+                // reference is.  They are rounded for the product, their sum is taken before, in 32 bits (the sum of the rounded ones would
+                // make one key alone exact, and costs two instructions more a key: 66 instead of 63 us for 32 trees).
+                const float most = tt_max3(tt_max3(mx[0], mx[1], mx[2]), tt_max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * c;
+                const float top = !begun || m == -INFINITY ? most : most > m + 8.f ? most : m;
+                if (begun && __any_sync(0xffffffffu, top != m)) {
+                    // O with the turn's last product in it (those before it came ahead of these scores)
+                    const float keep = m == -INFINITY ? 0.f : at_exp2(m - top);
+                    l *= keep;
+                    ok = at_mbar_wait_warp(&o_done[turn], (taken + 1) & 1, failed);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+                    for (int d = 0; d < D; d += 16) {
+                        uint32_t y[16];
+                        tt_ld16_nowait(tO + d, y);
+                        tt_wait_ld16(y);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) y[j] = __float_as_uint(__uint_as_float(y[j]) * keep);
+                        at_tmem_st16(tO + d, y);
+                    }
+                }
+                m = top;
+                begun = true;
+                if (paired) TT_SYNC(turn * 4 + qd);
+                const float2 c2 = make_float2(c, c), minus = make_float2(m == -INFINITY ? 0.f : -m, m == -INFINITY ? 0.f : -m);
+                float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                // P over its scores (they are in registers), two keys a column
+                uint32_t pk[32];
+#pragma unroll
+                for (int j = 0; j < 64; j += 2) {
+                    const float2 e = tt_fma2(make_float2(__uint_as_float(x[j >> 5][j & 31]), __uint_as_float(x[j >> 5][(j & 31) + 1])), c2, minus);
+                    const float2 w2 = make_float2(at_exp2(e.x), at_exp2(e.y));
+                    sums[(j >> 1) & 1] = tt_add2(sums[(j >> 1) & 1], w2);
+                    pk[j >> 1] = pack_bf16(w2.x, w2.y);
+                }
+                at_tmem_st32(tB, pk);
+                if (paired) {
+                    --left;
+                    if (turn == 0 || left > 0) TT_ARRIVE((turn ^ 1) * 4 + qd);
+                }
+                const float2 sum = tt_add2(sums[0], sums[1]);
+                l += sum.x + sum.y;
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) at_mbar_arrive(&p_ready[turn * 2 + buffer]);
+            }
+            while (left > 0) {                                  // (a tile fewer, or given up)
+                TT_SYNC(turn * 4 + qd);
+                --left;
+                if (turn == 0 || left > 0) TT_ARRIVE((turn ^ 1) * 4 + qd);
+            }
             // ---- the unit's end, or the share's
             float f0 = 1.f, f1 = 0.f;
             if (!dual) {                                        // both turns' parts: each thread has half of the pair's columns
@@ -684,7 +736,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attention_tc_kernel(const 
                 continue;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const bool two = !dual && g.upto - g.from > 1, bad = odd[seg & 3] == (seg & 0xff) + 1 && g.upto == g.tiles;
+            const bool two = !dual && g.upto - g.from > 1, bad = odd[seg & 15] == (seg & 0xff) + 1;
             const int col0 = dual ? 0 : turn * (D / 2), cols = dual ? D : D / 2;
             const float inv = l == 0.f ? 0.f : 1.f / l;
             float* po = a.parts + (size_t)(2 * blockIdx.x + (g.from == 0 ? 1 : 0)) * (D * TT_UNIT);

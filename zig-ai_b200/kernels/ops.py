@@ -1449,10 +1449,12 @@ def tree_attention(q, k, v, step, cache, heads, kv_heads, head_dim, scale, windo
     if impl == "mma" and not mma:
         raise KernelError("tree_attention: the tensor-core kernel takes bfloat16 heads of 32, 64, 96 or 128 on 16-byte boundaries")
     width = bt.shape[1] * cache.page_size
-    # Trees of more than 32 pairs of a row and a query head over many keys: tcgen05 (us, tcgen05 and mma.sync: 32 trees of 4-24 rows of 32 heads over 8
-    # behind 300-6000 positions 96 and 148, 8 of 16 rows behind 2000 27 and 28; few pairs and few keys: 8 of 8 rows 25 and 20, one of 12
-    # rows behind 1000 positions 19 and 12)
-    tc = (mma and impl != "mma" and window is None and most <= 128 and (impl == "tcgen05" or (most * group > 32 and S * G * width >= 16384))
+    # tcgen05 where a request's keys are many for its pairs of a row and a query head (us, mma.sync and tcgen05, 32 heads over 8 unless it says otherwise:
+    # 132 pairs behind 0 positions 9 and 12; 64 requests of 68 pairs behind 100 positions 48 and 38; one of 128 behind 500 24 and 14; 64
+    # of 36 behind 300 33 and 40; 8 of 64 behind 1000 21 and 19; 16 of 32 behind 1000 20 and 23; 8 of 32 behind 8000 43 and 36; one of 16
+    # behind 30 000 36 and 24; 32 of 16 behind 4000 61 and 62, with heads of 128 102 and 93; one of 256 behind 30 000, heads of 128, 268 and 52)
+    long = width >= (256 if most * group > 64 else 1024 if most * group > 32 else 4096)
+    tc = (mma and impl != "mma" and window is None and most <= 128 and (impl == "tcgen05" or long)
           and not (qp & 15 or qs & 7) and bool(_fn("tree_attention_tc", "zai_tree_attention_tc_supports")(D, cache.page_size, pages.shape[0], G)))
     if impl == "tcgen05" and not tc:
         raise KernelError("tree_attention: the tcgen05 kernel takes bfloat16 heads of 64 or 128 on 16-byte boundaries, trees of at most 128 rows, no window")
