@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(GEN_THREADS) tree_attention_general_kernel(con
     float* ring = qs + GEN_PAIRS * D4;                         // [stages][stage]
     float* ps = ring + stages * stage;                         // [4 warps][32 keys][4 pairs]
     float* ml = ps + GEN_PAIRS * GEN_KEYS;                     // [16][2]
-    const T** where = reinterpret_cast<const T**>(ml + 2 * GEN_PAIRS);     // [2][32][key, value]
+    const T** where = reinterpret_cast<const T**>(ml + 2 * GEN_PAIRS);     // [4][32][key, value]
     pdl_trigger();
     pdl_wait();
     const Tile t = find_tile(a, blockIdx.x / splits, GEN_PAIRS, blockIdx.x / splits == gridDim.x / splits - 1);
@@ -146,8 +146,8 @@ __global__ void __launch_bounds__(GEN_THREADS) tree_attention_general_kernel(con
     const int from = (int)((long long)total * rank / splits), upto = (int)((long long)total * (rank + 1) / splits);
     const ZaiTableRow table = {a.table + (size_t)t.s * a.table_width, a.table_width, a.num_pages, a.status};
 
-    auto look_up = [&](int it) {                               // where tile `it`'s keys lie, by the last warp
-        if (warp != GEN_THREADS / 32 - 1 || it >= upto) return;
+    auto look_up = [&](int it, int by) {                       // where tile `it`'s keys lie, by one warp
+        if (warp != by || it >= upto) return;
         const T *kp = nullptr, *vp = nullptr;
         if (it >= cached) {
             const int key = (it - cached) * GEN_KEYS + lane;
@@ -163,23 +163,31 @@ __global__ void __launch_bounds__(GEN_THREADS) tree_attention_general_kernel(con
                 vp = kp + (long long)a.G * a.page_size * D;
             }
         }
-        const T** w = where + ((it & 1) * GEN_KEYS + lane) * 2;
+        const T** w = where + ((it & 3) * GEN_KEYS + lane) * 2;
         w[0] = kp;
         w[1] = vp;
     };
+    // (a thread's pieces of 16 bytes of a tile, 128 apart: one division for all)
+    const int quads = D4 >> 2, key_at = threadIdx.x / quads, quad_at = threadIdx.x - key_at * quads, key_step = GEN_THREADS / quads;
+    const int quad_step = GEN_THREADS - key_step * quads;
     // tile `it` into its stage; keys that are not there become zeros.  Returns whether a value is not finite (ASYNC: not known here).
     auto bring = [&](int it) {
         bool odd = false;
         if (it < upto) {
             float *ks = ring + (it % stages) * stage, *vs = ks + GEN_KEYS * KS;
-            const T* const* w = where + (it & 1) * GEN_KEYS * 2;
+            const T* const* w = where + (it & 3) * GEN_KEYS * 2;
             if (ASYNC) {
-                const int quads = D >> 2;
-                for (int e = threadIdx.x; e < GEN_KEYS * quads; e += GEN_THREADS) {
-                    const int j = e / quads, c = (e - j * quads) * 4;
+                for (int j = key_at, q = quad_at; j < GEN_KEYS;) {
+                    const int c = q * 4;
                     const T *kp = w[2 * j], *vp = w[2 * j + 1];
                     cp_async16(ks + j * KS + c, kp ? (const void*)(kp + c) : a.pages, kp != nullptr);
                     cp_async16(vs + j * D4 + c, vp ? (const void*)(vp + c) : a.pages, vp != nullptr);
+                    j += key_step;
+                    q += quad_step;
+                    if (q >= quads) {
+                        q -= quads;
+                        ++j;
+                    }
                 }
             } else {
                 for (int e0 = threadIdx.x; e0 < GEN_KEYS * D; e0 += 4 * GEN_THREADS) {
@@ -207,22 +215,11 @@ __global__ void __launch_bounds__(GEN_THREADS) tree_attention_general_kernel(con
         if (ASYNC) cp_async_commit();
         return odd;
     };
-    for (int e = threadIdx.x; e < GEN_PAIRS * D4; e += GEN_THREADS) {
-        const int r = e / D4, d = e - r * D4, p = t.pair0 + r;
-        qs[e] = r < pairs && d < D ? to_float(((const T*)a.q)[(long long)(t.first + p / group) * a.q_stride + (head * group + p % group) * D + d]) : 0.f;
-    }
     if (D4 != D)                                               // the columns behind a key's own: zeros in every stage (never ASYNC)
         for (int e = threadIdx.x; e < stages * GEN_KEYS * (D4 - D); e += GEN_THREADS) {
             const int j = e / (D4 - D), c = D + e - j * (D4 - D);
             ring[(j / GEN_KEYS) * stage + (j % GEN_KEYS) * KS + c] = 0.f;
         }
-    int node[4], pos[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = warp * 4 + i;
-        node[i] = r < pairs ? (t.pair0 + r) / group : -1;
-        pos[i] = node[i] >= 0 && a.window > 0 ? a.positions[t.first + node[i]] : 0;
-    }
     float o[4][COLS], m[4], l[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -232,12 +229,23 @@ __global__ void __launch_bounds__(GEN_THREADS) tree_attention_general_kernel(con
         for (int c = 0; c < COLS; ++c) o[i][c] = 0.f;
     }
     const int ahead = ASYNC ? stages - 1 : 0;                  // tiles whose copies are on their way
-    for (int it = from; it < from + ahead; ++it) {
-        look_up(it);
-        __syncthreads();
-        bring(it);
+    // (the first tiles at once, each by a warp, and the queries while their copies are on their way)
+    for (int i = 0; i <= ahead; ++i) look_up(from + i, i);
+    __syncthreads();
+    for (int i = 0; i < ahead; ++i) bring(from + i);
+    int node[4], pos[4];                                       // this warp's pairs; their queries
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = warp * 4 + i, p = t.pair0 + r, at = p / group;
+        node[i] = r < pairs ? at : -1;
+        pos[i] = r < pairs && a.window > 0 ? a.positions[t.first + at] : 0;
+        const T* row = (const T*)a.q + (long long)(t.first + at) * a.q_stride + (head * group + p - at * group) * D;
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) {
+            const int d = lane + 32 * c;
+            if (d < D4) qs[r * D4 + d] = r < pairs && d < D ? to_float(row[d]) : 0.f;
+        }
     }
-    look_up(from + ahead);
     for (int it = from; it < upto; ++it) {
         const bool nodes = it >= cached;
         const int key0 = nodes ? (it - cached) * GEN_KEYS : (tile0 + it) * GEN_KEYS;
@@ -248,8 +256,8 @@ __global__ void __launch_bounds__(GEN_THREADS) tree_attention_general_kernel(con
             else cp_async_wait<0>();                           // (two stages: the only tile on its way)
             __syncthreads();                                   // (arrived, and the tile before has been used)
             bring(it + ahead);
-            look_up(it + ahead + 1);
-            if (nodes || a.window > 0) {                       // tiles that some pair sees in part
+            look_up(it + ahead + 1, GEN_THREADS / 32 - 1);
+            if (nodes || (a.window > 0 && key0 <= t.ctx + t.n - 1 - a.window)) {        // tiles that some pair sees in part
                 for (int e = lane; e < GEN_KEYS * D4; e += 32) odd |= !(fabsf(vs[e]) < INFINITY);
                 odd = __any_sync(0xffffffffu, odd);
             }
@@ -257,7 +265,7 @@ __global__ void __launch_bounds__(GEN_THREADS) tree_attention_general_kernel(con
             __syncthreads();                                   // (looked up, and the tile before has been used)
             odd = bring(it);
             odd = __syncthreads_or(odd);
-            look_up(it + 1);
+            look_up(it + 1, GEN_THREADS / 32 - 1);
         }
         // scores: this lane's key with the warp's pairs
         float s[4] = {0.f, 0.f, 0.f, 0.f};
@@ -280,8 +288,8 @@ __global__ void __launch_bounds__(GEN_THREADS) tree_attention_general_kernel(con
                                                      : key < t.ctx && (a.window <= 0 || key > pos[i] - a.window));
             const float x = seen ? s[i] * a.scale : -INFINITY;
             const float top = fmaxf(m[i], warp_max(x));
-            const float keep = top == -INFINITY ? 1.f : expf(m[i] - top);
-            const float p = seen ? expf(x - top) : 0.f;
+            const float keep = top == -INFINITY ? 1.f : fast_exp2((m[i] - top) * LOG2E);
+            const float p = seen ? fast_exp2((x - top) * LOG2E) : 0.f;
             l[i] = l[i] * keep + p;                            // (a lane's own keys; added up at the end)
             m[i] = top;
             wp[i] = p;
@@ -329,21 +337,26 @@ __global__ void __launch_bounds__(GEN_THREADS) tree_attention_general_kernel(con
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
     for (int r = rank + warp * splits; r < pairs; r += splits * (GEN_THREADS / 32)) {
-        float top = -INFINITY;
-        for (int i = 0; i < splits; ++i) top = fmaxf(top, cluster.map_shared_rank(ml, i)[2 * r]);
-        float sum = 0.f, x[COLS];
+        // (a lane a part: one after the other these trips to the other blocks' memory were most of the join)
+        float2 its = make_float2(-INFINITY, 0.f);
+        if (lane < splits) its = *reinterpret_cast<const float2*>(cluster.map_shared_rank(ml, lane) + 2 * r);
+        const float top = warp_max(its.y == 0.f ? -INFINITY : its.x), mine = its.y == 0.f ? 0.f : fast_exp2((its.x - top) * LOG2E), sum = warp_sum(mine * its.y);
+        float x[COLS];
 #pragma unroll
         for (int c = 0; c < COLS; ++c) x[c] = 0.f;
-        for (int i = 0; i < splits; ++i) {
-            const float* theirs = cluster.map_shared_rank(ml, i);
-            const float part = theirs[2 * r + 1];
-            if (part == 0.f) continue;                         // (a block that saw nothing of this pair)
-            const float f = expf(theirs[2 * r] - top);
-            const float* vals = cluster.map_shared_rank(po, i) + r * D;
-            sum += f * part;
+        for (int i0 = 0; i0 < splits; i0 += 4) {
+            float f[4], vals[4][COLS];
 #pragma unroll
-            for (int c = 0; c < COLS; ++c)
-                if (lane + 32 * c < D) x[c] += f * vals[lane + 32 * c];
+            for (int u = 0; u < 4; ++u) {
+                f[u] = i0 + u < splits ? __shfl_sync(0xffffffffu, mine, i0 + u) : 0.f;
+                const float* from_part = cluster.map_shared_rank(po, min(i0 + u, splits - 1)) + r * D;
+#pragma unroll
+                for (int c = 0; c < COLS; ++c) vals[u][c] = f[u] != 0.f && lane + 32 * c < D ? from_part[lane + 32 * c] : 0.f;
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)                        // (a block that saw nothing of this pair adds 0 times 0)
+#pragma unroll
+                for (int c = 0; c < COLS; ++c) x[c] = fmaf(f[u], vals[u][c], x[c]);
         }
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         const int p = t.pair0 + r;
@@ -428,6 +441,13 @@ __global__ void __launch_bounds__(32 * WM * WN) tree_attention_mma_kernel(const 
         cp_async_commit();
     };
 
+    static_assert(STAGES == 3, "two tiles on their way, a place for each");
+    // (the first tiles' places at once, and the queries while their copies are on their way)
+    look_up(from);
+    look_up(from + 1);
+    __syncthreads();
+    issue(from);
+    issue(from + 1);
     // this lane's two pairs: g and g + 8 of the warp's 16
     int node[2], pos[2];
     uint32_t qf[D / 16][4];
@@ -447,13 +467,8 @@ __global__ void __launch_bounds__(32 * WM * WN) tree_attention_mma_kernel(const 
                 qf[kk][i] = qr[i & 1] ? *reinterpret_cast<const uint32_t*>(qr[i & 1] + kk * 16 + (i >> 1) * 8) : 0u;
     }
     const bool idle = wm * 16 >= pairs;                        // a warp without pairs brings keys in and computes nothing
-    for (int it = from; it < from + STAGES - 1; ++it) {
-        look_up(it);
-        __syncthreads();
-        issue(it);
-    }
-    look_up(from + STAGES - 1);
-
+    __syncthreads();                                           // (the first two have been read)
+    look_up(from + 2);
     float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
     for (int d = 0; d < D / 8; ++d)
@@ -696,7 +711,7 @@ template <typename T, int COLS, bool ASYNC>
 static int launch_general(const TreeArgs& a, int tiles, int splits, cudaStream_t stream) {
     static unsigned long long done = 0;
     const size_t D4 = (a.D + 3) & ~3, stage = sizeof(float) * GEN_KEYS * (2 * D4 + 4);
-    const size_t rest = sizeof(float) * (GEN_PAIRS * D4 + GEN_PAIRS * GEN_KEYS + 2 * GEN_PAIRS) + sizeof(void*) * 4 * GEN_KEYS;
+    const size_t rest = sizeof(float) * (GEN_PAIRS * D4 + GEN_PAIRS * GEN_KEYS + 2 * GEN_PAIRS) + sizeof(void*) * 8 * GEN_KEYS;
     const int stages = !ASYNC ? 1 : 3 * stage + rest <= 76 * 1024 ? 3 : 2;      // (three of heads of up to 64, or two of 128: two blocks an SM and more)
     if (stages * stage + rest > 227 * 1024) return ZAI_BAD_SIZE;
     return launch_cluster(tree_attention_general_kernel<T, COLS, ASYNC>, &done, dim3((unsigned)splits * tiles, a.G), GEN_THREADS, stages * stage + rest,
