@@ -245,8 +245,9 @@ class Engine:
         """How likely the model finds given tokens: for every prompt a list with an entry for each token but the first: its log probability
         behind the tokens before it (`logprob`), its `rank` among all tokens (0: the likeliest), the `entropy` there in nats, and the
         `top` (at most 32) likeliest tokens with their log probabilities (`top`, pairs).  Runs beside requests that are being
-        served if slots and pages are free; prompts are cut into portions of `max_batched_tokens`."""
-        out, V = [], self.runner.model.vocab_size
+        served if slots and pages are free; prompts are cut into portions of `max_batched_tokens`, 2048 at most (all of a portion's
+        logits are in memory at once)."""
+        out, V, portion = [], self.runner.model.vocab_size, min(self.scheduler.max_batched_tokens, 2048)
         if not 0 <= int(top) <= min(32, V):
             raise ValueError(f"{top} alternatives of {V} tokens; at most 32")
         for k, prompt in enumerate(prompts):
@@ -257,8 +258,8 @@ class Engine:
                 raise ValueError(f"token ids {[t for t in tokens if not 0 <= t < V][:8]} are outside the vocabulary of {V}")
             self.runner.add_request(rid)
             try:
-                for a in range(0, len(tokens), self.scheduler.max_batched_tokens):
-                    part = tokens[a:a + self.scheduler.max_batched_tokens]
+                for a in range(0, len(tokens), portion):
+                    part = tokens[a:a + portion]
                     n = min(len(part), len(tokens) - 1 - a)             # (the last token has none behind it)
                     logits = self.runner.step([(rid, part, list(range(n)))])
                     if n == 0:
