@@ -757,3 +757,52 @@ def test_scores_beside_requests_that_are_served(tree_models):
         done[r.request_id] = r.output
     assert [done[i] for i in ids] == want_out
     eng.runner.cache.check()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("ps", [8, 32, 128, 256])
+def test_many_short_units(D, ps):
+    """Shares of many units of one to four tiles, of one turn's pairs and of both turns' in any order, cached lengths at every side of a tile's border."""
+    g, H, G = random.Random(ps + D), 8, 2
+    for shape in ("mixed", "forest"):
+        q_lens = [g.choice([0, 1, 2, 5, 31, 32, 33, 64, 65, 70, 128]) for _ in range(50)]
+        ctx = [g.choice([0, 1, 63, 64, 65, 127, 128, 130, 200]) for _ in range(50)]
+        q, k, v, step, cache, _ = make_tree_step(q_lens, ctx, H, G, D, ps, BF16, ps, shape, packed=shape == "mixed")
+        got = ops().tree_attention(q, k, v, step, cache, H, G, D, D ** -0.5, impl="tcgen05")
+        close(got, q, k, v, step, cache, H, G, D, D ** -0.5, None)
+        for _ in range(5):
+            assert torch.equal(ops().tree_attention(q, k, v, step, cache, H, G, D, D ** -0.5, impl="tcgen05"), got)
+    assert ops().read_status() == 0
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_what_is_not_finite_in_many_short_units(D):
+    """Of 60 units in a row every third has a drafted value that is not finite: the rows that see it end so in that column, the others as without it."""
+    g, H, G = random.Random(D), 8, 2
+    q_lens, ctx = [g.choice([3, 9, 40, 70]) for _ in range(60)], [g.choice([0, 5, 64, 100]) for _ in range(60)]
+    q, k, v, step, cache, parents = make_tree_step(q_lens, ctx, H, G, D, 16, BF16, 3)
+    want = ops().tree_attention(q, k, v, step, cache, H, G, D, 0.125, impl="tcgen05")
+    v = v.clone()
+    sees, hit, cu = ref_ops._bits(step.tree_mask, 70), torch.zeros((sum(q_lens), H, D), dtype=torch.bool, device="cuda"), 0
+    for s, n in enumerate(q_lens):
+        if s % 3 == 0:
+            row, head, col = g.randrange(n), g.randrange(G), g.randrange(D)
+            v[cu + row, head * D + col] = g.choice([float("nan"), float("inf")])
+            hit[cu:cu + n, head * (H // G):(head + 1) * (H // G), col] = sees[cu:cu + n, row][:, None]
+        cu += n
+    got = ops().tree_attention(q, k, v, step, cache, H, G, D, 0.125, impl="tcgen05").view(-1, H, D)
+    assert not torch.isfinite(got[hit]).any() and torch.equal(got[~hit], want.view(-1, H, D)[~hit])
+    assert ops().read_status() == 0
+
+
+@pytest.mark.parametrize("impl", ["general", "mma", "tcgen05"])
+@pytest.mark.parametrize("D,group,G", [(64, 3, 1), (128, 7, 2), (64, 1, 5), (128, 16, 1), (64, 40, 1)])
+def test_other_head_layouts_and_columns_of_one_projection(impl, D, group, G):
+    """q, k and v as columns of one product's rows; query heads that share a key/value head by threes, sevens and forties."""
+    H = group * G
+    q, k, v, step, cache, _ = make_tree_step([9, 1, 50], [70, 0, 300], H, G, D, 32, BF16, 4)
+    rows = torch.cat([q, k, v], 1)
+    q2, k2, v2 = rows[:, :H * D], rows[:, H * D:(H + G) * D], rows[:, (H + G) * D:]
+    got = ops().tree_attention(q2, k2, v2, step, cache, H, G, D, D ** -0.5, impl=impl)
+    close(got, q, k, v, step, cache, H, G, D, D ** -0.5, None)
+    assert torch.equal(got, ops().tree_attention(q, k, v, step, cache, H, G, D, D ** -0.5, impl=impl)) and ops().read_status() == 0
