@@ -9,6 +9,7 @@ cuBLAS through `torch.matmul`, as the reference sends every projection to `cubla
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import os
 import sys
@@ -1406,6 +1407,12 @@ def step_layout(q_lens, ctx_lens, slots, page_rows, page_size, n_rows, width, pa
     return StepLayout(*parts[:5], parts[5].view(S + 1, width), parts[6].view(N, words) if words else None)
 
 
+@functools.lru_cache(maxsize=None)
+def _tree_kernel_takes(fn, *sizes):
+    """What a tree-attention kernel says of these sizes (asked once: 1.2 us a question)."""
+    return _fn("tree_attention" if fn != "tc_supports" else "tree_attention_tc", "zai_tree_attention_" + fn)(*sizes)
+
+
 @_timed("attention")
 def tree_attention(q, k, v, step, cache, heads, kv_heads, head_dim, scale, window=None, impl=None, splits=None):
     """Attention of drafted rows: row i of a request sees the request's `step.ctx_lens` cached positions in the pages and those
@@ -1444,7 +1451,7 @@ def tree_attention(q, k, v, step, cache, heads, kv_heads, head_dim, scale, windo
     status, sms, stream = _place(index, "tree_attention")
     group, most = H // G, max(int(step.max_q_len), 1)
     qp, kp, vp, pp = q.data_ptr(), k.data_ptr(), v.data_ptr(), pages.data_ptr()
-    mma = (q.dtype == torch.bfloat16 and impl != "general" and bool(_fn("tree_attention", "zai_tree_attention_mma_supports")(D))
+    mma = (q.dtype == torch.bfloat16 and impl != "general" and _tree_kernel_takes("mma_supports", D)
            and not ((kp | vp | pp) & 15 or (ks | vs) & 7 or qp & 3 or qs & 1))
     if impl == "mma" and not mma:
         raise KernelError("tree_attention: the tensor-core kernel takes bfloat16 heads of 32, 64, 96 or 128 on 16-byte boundaries")
@@ -1455,7 +1462,7 @@ def tree_attention(q, k, v, step, cache, heads, kv_heads, head_dim, scale, windo
     # behind 30 000 36 and 24; 32 of 16 behind 4000 61 and 62, with heads of 128 102 and 93; one of 256 behind 30 000, heads of 128, 268 and 52)
     long = width >= (256 if most * group > 64 else 1024 if most * group > 32 else 4096)
     tc = (mma and impl != "mma" and window is None and most <= 128 and (impl == "tcgen05" or long)
-          and not (qp & 15 or qs & 7) and bool(_fn("tree_attention_tc", "zai_tree_attention_tc_supports")(D, cache.page_size, pages.shape[0], G)))
+          and not (qp & 15 or qs & 7) and _tree_kernel_takes("tc_supports", D, cache.page_size, pages.shape[0], G))
     if impl == "tcgen05" and not tc:
         raise KernelError("tree_attention: the tcgen05 kernel takes bfloat16 heads of 64 or 128 on 16-byte boundaries, trees of at most 128 rows, no window")
     if tc:
@@ -1469,7 +1476,7 @@ def tree_attention(q, k, v, step, cache, heads, kv_heads, head_dim, scale, windo
         while pairs < 128 and pairs < most * group:
             pairs *= 2
     else:
-        pairs = _fn("tree_attention", "zai_tree_attention_general_pairs")()
+        pairs = _tree_kernel_takes("general_pairs")
     tiles = S if most * group <= pairs else N * group // pairs + S
     if splits is None:
         # as many blocks to a tile's keys as fill the SMs about twice (us at 1, 4, 8 and 16: 8 trees of 8 rows behind 2000 positions 40, 20, 34, 78; one
