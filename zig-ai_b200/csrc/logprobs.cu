@@ -7,9 +7,9 @@
 // A thread keeps m, z, u of what it has seen (rescaled when its maximum grows) and the count for the rank; they are joined at the end.
 //
 // The best tokens.  An entry's key is its value's bits in an order that compares as a whole number, and behind them the complement
-// of its index: keys are all different, and the order of keys is the order wanted.  The first round of the walk is split into 32 groups by
-// lane; the top-th largest of the groups' largest keys bounds the row's top-th key from below (`top` <= 32), so only keys at or above it are noted in
-// shared memory: some thirty of each 4096 entries.  After 4, 8, 16, .. rounds the list is cut down to the `top` largest, the last of which is the new bound,
+// of its index: keys are all different, and the order of keys is the order wanted.  The first round of the walk is split into 64 groups by
+// lane and half of the block; the top-th largest of the groups' largest keys bounds the row's top-th key from below (`top` <= 32), so only keys at or above it are noted in
+// shared memory: some twenty of each 4096 entries.  After 2, 4, 8, 16, .. rounds the list is cut down to the `top` largest, the last of which is the new bound,
 // so that as many rounds again note as many again.  A key's place is the number of noted keys above it.  A row that
 // notes more than there is room for (one that ascends) is walked again in steps that cut the list down as they go.
 //
@@ -18,8 +18,8 @@
 // keys to note only where its round's maximum reaches the bound, and 0 times -inf, which only masked tokens bring, is put right afterwards.
 //
 // A row is split over a cluster of up to 16 blocks when there are few rows; the first block joins the parts through distributed shared memory.
-// Measured: 2048 rows of 64 401 in 32 bits 87 us without alternatives (6.1 TB/s), 112 with 5, 152 with 20; in bfloat16 2048 of 65 536 82, 116 and 153.
-// 8 rows of 65 536 with 20 alternatives 11 us: two rounds a block, the candidates' counts, the join.
+// Measured: 2048 rows of 64 401 in 32 bits 87 us without alternatives (6.1 TB/s), 103 with 5, 121 with 20, 139 with 32; in
+// bfloat16 86, 115 and 133 (2048 of 65 536).  8 rows of 65 536 with 20 alternatives 10 us: two rounds a block, the candidates' counts, the join.
 #include <cooperative_groups.h>
 #include "common.cuh"
 namespace cg = cooperative_groups;
@@ -28,7 +28,6 @@ namespace cg = cooperative_groups;
 #define LP_WARPS (LP_THREADS / 32)
 #define LP_ROUND 16                 // entries of a row a thread looks at in one round
 #define LP_ROOM 1024                // noted keys a block has room for
-#define LP_PART 64                  // noted keys a block of a cluster may hand on (16 blocks: LP_ROOM)
 typedef unsigned long long u64;
 
 __device__ __forceinline__ u64 key_of(float x, int j) {
@@ -169,7 +168,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_kernel(float* __
         const int* __restrict__ targets, int V, int top, int blocks, int* status) {
     constexpr int VEC = Piece<T>::VEC;
     __shared__ u64 list[TOP ? LP_ROOM : 1];
-    __shared__ u64 best[32], groups[TOP ? 32 : 1];
+    __shared__ u64 best[32], groups[TOP ? 64 : 1];
     __shared__ u64 warp_best[TOP ? LP_THREADS : 1];
     __shared__ u64 bound_s;
     __shared__ int noted;
@@ -210,21 +209,30 @@ __global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_kernel(float* __
 #pragma unroll
         for (int e = 0; e < LP_ROUND; e += 4) top4[e / 4] = fmaxf(max3(x[e], x[e + 1], x[e + 2]), x[e + 3]);
         top_x = fmaxf(max3(top4[0], top4[1], top4[2]), top4[3]);
-        if (TOP && (top_x >= bound_x || top_x != top_x)) {
-#pragma unroll
-            for (int e4 = 0; e4 < LP_ROUND; e4 += 4) {
-                if (!(top4[e4 / 4] >= bound_x) && bound_x != -INFINITY) continue;
-#pragma unroll
-                for (int e = e4; e < e4 + 4; ++e)
-                    if (x[e] >= bound_x || x[e] != x[e]) {
-                        const int j = index_in_round<T>(at, e);
-                        const u64 k = key_of(x[e], j - lead);
-                        if (k >= bound && j >= lo && j < hi) {
-                            const int p = atomicAdd(&noted, 1);
-                            if (p < LP_ROOM) list[p] = k;
-                        }
-                    }
-            }
+        if (TOP) {
+            // (the entries of the lanes that have such a key are looked at once more, in memory, by few instructions: with the registers' sixteen
+            // copies of this code it was a third of the kernel, most of it their own arrival)
+            auto note = [&](int j) {
+                if (j < lo || j >= hi) return;
+                const u64 k = key_of(to_float(base[j]), j - lead);
+                if (k < bound) return;
+                const int p = atomicAdd(&noted, 1);
+                if (p < LP_ROOM) list[p] = k;
+            };
+            unsigned hits = __ballot_sync(0xffffffffu, top_x >= bound_x || top_x != top_x);
+            if (__popc(hits) > 8)
+#pragma unroll 1
+                for (int e = 0; e < LP_ROUND; ++e) note(index_in_round<T>(at, e));
+            else
+#pragma unroll 1
+                while (hits) {                                 // two lanes' sixteen entries at a time
+                    const int one = __ffs(hits) - 1;
+                    hits &= hits - 1;
+                    const int two = __ffs(hits) - 1, of = lane < LP_ROUND ? one : two, e = lane & (LP_ROUND - 1);
+                    hits &= hits - 1;
+                    if (of >= 0) note(at + ((e / VEC) * LP_THREADS + warp * 32 + of) * VEC + e % VEC);
+                    __syncwarp();
+                }
         }
         if (top_x > mine.m) {
             const Sums none = {top_x, 0.f, 0.f};
@@ -291,14 +299,17 @@ __global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_kernel(float* __
             }
         warp_best[t] = k;
         __syncthreads();
-        if (warp == 0) {
+        if (warp < 2) {                                        // (64 groups: a lane of either half of the warps)
+            k = 0;
 #pragma unroll
-            for (int w = 1; w < LP_WARPS; ++w) k = max(k, warp_best[w * 32 + lane]);
-            groups[lane] = k;
-            __syncwarp();
+            for (int w = 0; w < LP_WARPS / 2; ++w) k = max(k, warp_best[(warp * (LP_WARPS / 2) + w) * 32 + lane]);
+            groups[t] = k;
+        }
+        __syncthreads();
+        if (warp < 2) {
             int above = 0;
 #pragma unroll 8
-            for (int i = 0; i < 32; ++i) above += groups[i] > k || (groups[i] == k && i < lane);   // (groups without entries are equal)
+            for (int i = 0; i < 64; ++i) above += groups[i] > k || (groups[i] == k && i < t);      // (groups without entries are equal)
             if (above == top - 1) bound_s = k;
         }
         __syncthreads();
@@ -312,8 +323,8 @@ __global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_kernel(float* __
             round(y, at + step);
             if (at + 3 * step < hi) load_round<T>(base, at + 3 * step, lo, hi, y);
         }
-        if (TOP && (number & (number - 1)) == 0 && number >= 4 && at + 3 * step < hi) {
-            // after 4, 8, 16, .. rounds: the list cut down to the largest so far, and the bound raised
+        if (TOP && (number & (number - 1)) == 0 && at + 2 * step < hi) {
+            // after 2, 4, 8, 16, .. rounds: the list cut down to the largest so far, and the bound raised
             __syncthreads();
             const int n = noted;
             __syncthreads();
@@ -374,7 +385,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_kernel(float* __
             if (t == 0) bound_s = bound;
             __syncthreads();
         }
-        if (blocks > 1 && noted > LP_PART) {
+        if (blocks > 1 && noted > top) {                       // (the row's bound is then the highest of the blocks' own: few keys are handed on)
             select_largest(list, noted, top, best);
             if (t < top) list[t] = best[t];
             if (t == 0) {
