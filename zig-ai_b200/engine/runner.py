@@ -223,18 +223,24 @@ class ModelRunner:
                 raise StepError(f"request {rid!r}: a tree of {len(tokens)} tokens")
         spans, tables = self._reserve([(rid, tokens, []) for rid, tokens, _ in entries])
         n = sum(len(t) for _, t, _ in entries)
-        pad = 0 if n <= 16 or self.device.type != "cuda" else -n % (32 if n <= 256 else 64)      # (few distinct row counts: see `pad_rows`)
-        step, tokens, parents, layouts = lay_out_trees(ops, self.dtype, self.device, spans, [p for _, _, p in entries], tables, self.cache.page_size, n + pad)
-        logits = self.model.forward(step, self.cache)
-        choices = torch.zeros_like(tokens)
-        chosen = (choose or ops.argmax)(logits)
-        if tuple(chosen.shape) != (n,):
-            raise StepError(f"{n} rows want a choice each, got {tuple(chosen.shape)}")
-        choices[:n] = chosen
-        accepted = ops.accept_drafts(choices, tokens, parents, step, step.max_q_len)
-        for k, v, group, pages in step.drafted:
-            ops.commit_drafts(k, v, accepted.path, accepted.counts, layouts[group], pages)
-        counts, chosen = accepted.counts.tolist(), accepted.tokens.tolist()
+        try:
+            pad = 0 if n <= 16 or self.device.type != "cuda" else -n % (32 if n <= 256 else 64)      # (few distinct row counts: see `pad_rows`)
+            step, tokens, parents, layouts = lay_out_trees(ops, self.dtype, self.device, spans, [p for _, _, p in entries], tables, self.cache.page_size, n + pad)
+            logits = self.model.forward(step, self.cache)
+            choices = torch.zeros_like(tokens)
+            chosen = (choose or ops.argmax)(logits)
+            if tuple(chosen.shape) != (n,):
+                raise StepError(f"{n} rows want a choice each, got {tuple(chosen.shape)}")
+            choices[:n] = chosen
+            accepted = ops.accept_drafts(choices, tokens, parents, step, step.max_q_len)
+            for k, v, group, pages in step.drafted:
+                ops.commit_drafts(k, v, accepted.path, accepted.counts, layouts[group], pages)
+            counts, chosen = accepted.counts.tolist(), accepted.tokens.tolist()
+        except BaseException:
+            # (nothing was kept: the positions reserved for the trees hold no tokens, and a window must not count them as seen)
+            for rid, _, _ in entries:
+                self.cache.settle(rid, self.processed[rid])
+            raise
         out = []
         for (rid, _, _), m, row in zip(entries, counts, chosen):
             self.processed[rid] += m
