@@ -128,3 +128,34 @@ def test_trees_in_windowed_layers_give_the_tokens_of_single_steps(dirs):
         last = out[-1]
     assert out == want["r2"][:len(out)]
     assert ref_ops.read_status() == 0
+
+
+def test_a_raised_status_word_is_read_before_the_counts_are_used(dirs):
+    """A step whose kernels raised the status word accepts nothing: lengths stay, whatever the counts say, and the next step is not blamed."""
+    for counts in (None, 99, -3):
+        r = runner(dirs["full"])
+        for rid in "ab":
+            r.add_request(rid)
+            r.step([(rid, [1, 2, 3], [])])
+
+        class Ops:
+            def __getattr__(self, name):
+                return getattr(ref_ops, name)
+
+            def accept_drafts(self, *a):
+                out = ref_ops.accept_drafts(*a)
+                ref_ops._raise(64)
+                return out if counts is None else out._replace(counts=torch.full_like(out.counts, counts))
+
+            def commit_drafts(self, *a):
+                pass
+
+        r.ops = Ops()
+        steps = r.steps
+        with pytest.raises(StepError, match=f"step {steps}: .*status 64.*void"):
+            r.verify([("a", [4, 5], [-1, 0]), ("b", [6, 5, 4], [-1, 0, 0])])
+        for rid in "ab":
+            holds(r, rid, 3)
+        r.ops = ref_ops
+        assert ref_ops.read_status() == 0
+        assert all(r.verify([("a", [4], [-1]), ("b", [6], [-1])]))

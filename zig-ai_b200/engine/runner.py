@@ -236,6 +236,9 @@ class ModelRunner:
             for k, v, group, pages in step.drafted:
                 ops.commit_drafts(k, v, accepted.path, accepted.counts, layouts[group], pages)
             counts, chosen = accepted.counts.tolist(), accepted.tokens.tolist()
+            self.steps += 1
+            self.tokens_run += n
+            self.check_status(self.steps - 1)                  # (before anything goes by what the kernels said)
         except BaseException:
             # (nothing was kept: the positions reserved for the trees hold no tokens, and a window must not count them as seen)
             for rid, _, _ in entries:
@@ -246,9 +249,6 @@ class ModelRunner:
             self.processed[rid] += m
             self.cache.settle(rid, self.processed[rid])
             out.append(row[:m])
-        self.steps += 1
-        self.tokens_run += n
-        self.check_status(self.steps - 1)
         return out
 
 
