@@ -258,12 +258,10 @@ class Engine:
                 raise ValueError(f"token ids {[t for t in tokens if not 0 <= t < V][:8]} are outside the vocabulary of {V}")
             self.runner.add_request(rid)
             try:
-                for a in range(0, len(tokens), portion):
-                    part = tokens[a:a + portion]
-                    n = min(len(part), len(tokens) - 1 - a)             # (the last token has none behind it)
+                for a in range(0, len(tokens) - 1, portion):
+                    part = tokens[a:min(a + portion, len(tokens) - 1)]      # (the last token has none behind it)
+                    n = len(part)
                     logits = self.runner.step([(rid, part, list(range(n)))])
-                    if n == 0:
-                        continue
                     targets = torch.tensor(tokens[a + 1:a + 1 + n], dtype=torch.int32, device=logits.device)
                     got = [t.tolist() for t in self.runner.ops.token_logprobs(logits, targets, top)]
                     entries += [dict(token=t, logprob=lp, rank=r, entropy=e, top=list(zip(ids, lps)))
