@@ -30,3 +30,25 @@ def test_only_tokens_that_something_is_read_behind_are_run(model_dir):
         assert (eng.runner.steps - before[0], eng.runner.tokens_run - before[1]) == (steps, n - 1)
     assert not eng.runner.processed
     eng.runner.cache.check()
+
+
+def test_scored_portions_make_no_step_graphs(model_dir):
+    """A graph of a scored portion would keep logits of every row (2048 x 65 536 in 32 bits: half a GB) and push out those of served steps."""
+    eng = engine(model_dir)
+
+    class Graphs:
+        asked = 0
+
+        def bucket(self, n):
+            return None
+
+        def run(self, spans, tables):
+            Graphs.asked += 1
+
+    want = eng.score([list(range(20))] * 2, top=2)
+    r = eng.runner
+    r.use_graphs, r.graphs, r.shape_graphs = True, Graphs(), Graphs()
+    assert eng.score([list(range(20))] * 2, top=2) == want and Graphs.asked == 0
+    r.add_request("a")
+    r.step([("a", [1, 2, 3], [2])])
+    assert Graphs.asked == 1

@@ -261,7 +261,7 @@ class Engine:
                 for a in range(0, len(tokens) - 1, portion):
                     part = tokens[a:min(a + portion, len(tokens) - 1)]      # (the last token has none behind it)
                     n = len(part)
-                    logits = self.runner.step([(rid, part, list(range(n)))])
+                    logits = self.runner.step([(rid, part, list(range(n)))], shape_graphs=False)
                     targets = torch.tensor(tokens[a + 1:a + 1 + n], dtype=torch.int32, device=logits.device)
                     got = [t.tolist() for t in self.runner.ops.token_logprobs(logits, targets, top)]
                     entries += [dict(token=t, logprob=lp, rank=r, entropy=e, top=list(zip(ids, lps)))

@@ -163,7 +163,7 @@ class ModelRunner:
                             f"{self.ops.describe_status(code)} (status {code}); its results are void")
 
     def step(self, entries, trusted: bool = False, device_tokens: Optional[torch.Tensor] = None,
-             check: bool = True) -> torch.Tensor:
+             check: bool = True, shape_graphs: bool = True) -> torch.Tensor:
         """entries: (request, its next tokens, wanted places among them).  Returns 32-bit logits
         [wanted, vocab] in the order of the entries and of their wanted places.  (A step that ran
         as a CUDA graph returns a view of that graph's output buffer, valid until the next such step.)
@@ -171,7 +171,10 @@ class ModelRunner:
         order of the entries; the tokens in `entries` are then placeholders.
         `check`: read the kernels' status word after the step and raise `StepError` if it is raised
         (this waits for the step; a caller that reads the word with its own results, as `Engine`
-        does in the copy that brings the token ids back, passes False)."""
+        does in the copy that brings the token ids back, passes False).
+        `shape_graphs`: let a step that is not of single tokens run as a graph of its shape, or earn one.  A graph keeps its
+        output, so a caller that wants the logits of every row (`Engine.score`) passes False: that would be half a GB for 2048 rows
+        of 65 536, beside the graphs that serving steps use."""
         spans, tables = self._reserve(entries, trusted)
         n_tokens = sum(len(e[1]) for e in entries)
         graphed = (self.use_graphs and n_tokens == len(entries) and self.graphs.bucket(len(entries)) is not None
@@ -186,7 +189,7 @@ class ModelRunner:
             else:
                 logits = full[torch.tensor(keep, dtype=torch.long, device=self.device)] if keep else full[:0]
         else:
-            logits = self.shape_graphs.run(spans, tables) if self.use_graphs else None
+            logits = self.shape_graphs.run(spans, tables) if self.use_graphs and shape_graphs else None
             if logits is None:
                 spans, tables = self._pad_rows(spans, tables)
                 batch = pack_step(self.ops, self.dtype, self.device, spans, tables, pin=True)
