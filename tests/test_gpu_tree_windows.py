@@ -106,3 +106,26 @@ def test_the_same_call_gives_the_same_bits(D, dtype, impl):
         ops().tree_attention(*other[:5], H, G, D, D ** -0.5, impl=impl)
         assert torch.equal(ops().tree_attention(q, k, v, step, cache, H, G, D, D ** -0.5, impl=impl), want)
     assert ops().read_status() == 0
+
+
+@pytest.mark.parametrize("dtype,impl", [(F32, None), (BF16, "general"), (BF16, "mma"), (BF16, "tcgen05")])
+@pytest.mark.parametrize("cu", [[0, 5, 7], [1, 5, 8], [0, 6, 4, 8], [0, 0], [0, 8, 7]])
+def test_rows_of_no_span_raise_the_status_word(dtype, impl, cu):
+    """A row that no span holds has no output, and a span of fewer than no rows is none: the step is void, and says so."""
+    q, k, v, step, cache, _ = make_tree_step([5, 3], [20, 130], 4, 2, 64, 16, dtype, 9)
+    S = len(cu) - 1
+    step.cu_q, step.n_seqs, step.max_q_len = torch.tensor(cu, dtype=torch.int32, device="cuda"), S, 8
+    step.ctx_lens, cache.block_table = step.ctx_lens[[0, 1, 1][:S]].contiguous(), cache.block_table[[0, 1, 1][:S]].contiguous()
+    ops().tree_attention(q, k, v, step, cache, 4, 2, 64, 0.125, impl=impl)
+    assert ops().read_status() == 32
+
+
+@pytest.mark.parametrize("S", [1, 31, 32, 33, 64, 65, 100])
+@pytest.mark.parametrize("dtype,impl", [(F32, None), (BF16, "mma"), (BF16, "tcgen05")])
+def test_spans_without_rows_at_both_ends_are_no_fault(S, dtype, impl):
+    """Rows in one span among many: the others hold none, and every row is in a span."""
+    for at in {0, S // 2, S - 1}:
+        q, k, v, step, cache, _ = make_tree_step([0] * at + [7] + [0] * (S - 1 - at), [33] * S, 4, 2, 64, 16, dtype, 9)
+        got = ops().tree_attention(q, k, v, step, cache, 4, 2, 64, 0.125, impl=impl)
+        assert ops().read_status() == 0
+        close(got, q, k, v, step, cache, 4, 2, 64, 0.125, None)

@@ -97,7 +97,7 @@ enum ZaiStatusBit {
     ZAI_ST_PAGE = 4,        // a block-table entry outside the pool
     ZAI_ST_SLOT = 8,        // a state slot outside the slots
     ZAI_ST_POSITION = 16,   // a position outside the request's block-table row
-    ZAI_ST_ROWS = 32,       // spans of more rows than the step has room for, a row outside the step
+    ZAI_ST_ROWS = 32,       // spans that hold more rows than the step has room for or (where every row has to be in one) fewer, a row outside the step
     ZAI_ST_TREE = 64        // a drafted row whose parent is not before it, a tree of more rows than it may have
 };
 __device__ __forceinline__ void zai_raise(int* status, int bit) {

@@ -48,11 +48,12 @@ __device__ __forceinline__ Tile find_tile(const TreeArgs& a, int number, int M, 
         int first = 0, n = 0;
         if (s < a.S) {
             first = a.cu[s];
-            n = a.cu[s + 1] - first;
-            if (n > 0 && (first < 0 || first + n > a.N)) {     // (rows outside the step: the span is passed over)
-                zai_raise(a.status, ZAI_ST_ROWS);
-                n = 0;
-            }
+            const int end = a.cu[s + 1];
+            n = end - first;
+            // (rows outside the step, or fewer than none: the span is passed over; rows before the first span or behind the last one, which
+            // the last tile's block gets to see in any case: nobody computes them)
+            if (first < 0 || end < first || end > a.N) n = 0;
+            if (first < 0 || end < first || end > a.N || (s == 0 && first != 0) || (s == a.S - 1 && end != a.N)) zai_raise(a.status, ZAI_ST_ROWS);
         }
         const int tiles = n > 0 ? (n * group + M - 1) / M : 0;
         int upto = tiles;

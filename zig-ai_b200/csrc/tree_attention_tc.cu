@@ -61,14 +61,12 @@ __device__ __forceinline__ int unit_cost(const TtArgs& a, int pairs) { return pa
 __device__ __forceinline__ Request request_of(const TtArgs& a, int s, bool say) {
     Request r = {0, 0, 0, 0, 0, 0, 0};
     r.first = a.cu[s];
-    r.n = a.cu[s + 1] - r.first;
+    const int end = a.cu[s + 1];
+    r.n = end - r.first;
     r.ctx = max(a.ctx[s], 0);
-    if (r.n <= 0) {
-        r.n = 0;
-        return r;
-    }
-    if (r.first < 0 || r.first + r.n > a.N) {
-        if (say) zai_raise(a.status, ZAI_ST_ROWS);
+    const bool outside = r.first < 0 || end < r.first || end > a.N;     // (the span is passed over; rows before the first span or behind the last: nobody's)
+    if (say && (outside || (s == 0 && r.first != 0) || (s == a.S - 1 && end != a.N))) zai_raise(a.status, ZAI_ST_ROWS);
+    if (outside || r.n == 0) {
         r.n = 0;
         return r;
     }

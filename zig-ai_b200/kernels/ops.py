@@ -629,7 +629,7 @@ USE_TC_GEMM = os.environ.get("ZAI_TC_GEMM", "0") == "1"
 # with them and throws the step away if it is not zero.
 STATUS_BITS = {1: "a bounded wait inside a kernel ran out", 2: "a token id outside the vocabulary",
                4: "a block-table entry outside the page pool", 8: "a state slot outside the slots",
-               16: "a position outside its request's block-table row", 32: "spans of more rows than the step has, or a row outside it",
+               16: "a position outside its request's block-table row", 32: "spans that hold more rows than the step has or fewer, or a row outside it",
                64: "a drafted row whose parent is not before it, or a tree of too many rows"}
 _status = {}
 
@@ -1419,8 +1419,8 @@ def tree_attention(q, k, v, step, cache, heads, kv_heads, head_dim, scale, windo
     rows of its own span whose bit stands in `step.tree_mask` [N, words] (int32; as `step_layout` makes it); keys and values of
     the step's rows are k and v [N, kv_heads * head_dim] (columns of the projection's rows are fine) and enter no page:
     `commit_drafts` caches those that are accepted.  `window`: of all these, the ones whose position is above the row's minus the
-    window (`step.positions`: ctx plus the row's depth).  A row that sees nothing gets zeros.  `step.max_q_len` bounds all spans, that of
-    no request among them; a longer one raises the status word.  `impl`: "general", "mma" or "tcgen05" (None: by the sizes); `splits`:
+    window (`step.positions`: ctx plus the row's depth).  A row that sees nothing gets zeros.  The spans hold all N rows, and `step.max_q_len`
+    bounds all of them, that of no request among them; a row of no span, or a longer span, raises the status word.  `impl`: "general", "mma" or "tcgen05" (None: by the sizes); `splits`:
     how many blocks share a tile's keys in the first two (None: by the sizes)."""
     if impl not in (None, "general", "mma", "tcgen05"):
         raise KernelError(f"tree_attention: no kernel {impl!r}")
