@@ -129,3 +129,19 @@ def test_spans_without_rows_at_both_ends_are_no_fault(S, dtype, impl):
         got = ops().tree_attention(q, k, v, step, cache, 4, 2, 64, 0.125, impl=impl)
         assert ops().read_status() == 0
         close(got, q, k, v, step, cache, 4, 2, 64, 0.125, None)
+
+
+def test_sizes_beyond_32_bits_keep_their_meaning():
+    """A window of 2^32 + 5 positions is no window of five; tables are not laid out for a page size or a row count that wraps."""
+    o = ops()
+    for dtype, impl in ((F32, None), (BF16, "mma")):
+        q, k, v, step, cache, _ = make_tree_step([5, 3], [20, 130], 4, 2, 64, 16, dtype, 9)
+        want = o.tree_attention(q, k, v, step, cache, 4, 2, 64, 0.125, 0x7fffffff, impl=impl, splits=2)
+        close(want, q, k, v, step, cache, 4, 2, 64, 0.125, None)
+        for window in (1 << 31, (1 << 32) + 5, 1 << 40):
+            assert torch.equal(o.tree_attention(q, k, v, step, cache, 4, 2, 64, 0.125, window, impl=impl, splits=2), want)
+    one, rows = torch.ones(1, dtype=torch.int32, device="cuda"), torch.ones((2, 3), dtype=torch.int32, device="cuda")
+    for kw in (dict(page_size=(1 << 32) + 4), dict(n_rows=1 << 32), dict(width=(1 << 32) + 1)):
+        with pytest.raises(o.KernelError):
+            o.step_layout(**{**dict(q_lens=one, ctx_lens=one, slots=one, page_rows=rows, page_size=4, n_rows=1, width=2), **kw})
+    assert o.read_status() == 0

@@ -1390,7 +1390,7 @@ def step_layout(q_lens, ctx_lens, slots, page_rows, page_size, n_rows, width, pa
     its ancestors and itself.  Rows behind the last span belong to a span of no request: the null page, slot -1, nothing seen."""
     index = _int32("step_layout", q_lens, ctx_lens, slots, page_rows, *(() if parents is None else (parents,)))
     S, N, width, tree_rows = q_lens.numel(), int(n_rows), int(width), int(tree_rows) if parents is not None else 0
-    if N < 0 or width < 1 or int(page_size) < 1:
+    if not 0 <= N <= 0x7fffffff or not 1 <= width <= 0x7fffffff or not 1 <= int(page_size) <= 0x7fffffff:
         raise KernelError(f"step_layout: {N} rows, block tables of {width} pages of {page_size} positions")
     if ctx_lens.shape != q_lens.shape or slots.shape != q_lens.shape or q_lens.dim() != 1 or page_rows.dim() != 2:
         raise KernelError("step_layout: one length, one context and one slot a request, and the slots' block tables as rows")
@@ -1484,7 +1484,7 @@ def tree_attention(q, k, v, step, cache, heads, kv_heads, head_dim, scale, windo
         splits, keys = 1, width if window is None else min(width, int(window))
         while splits < 16 and splits * 64 < keys and tiles * G * splits < 256:
             splits *= 2
-    tail = (tiles, int(splits), cache.page_size, pages.shape[0], H, G, D, scale, int(window or 0), status, stream)
+    tail = (tiles, int(splits), cache.page_size, pages.shape[0], H, G, D, scale, min(int(window or 0), 0x7fffffff), status, stream)
     if mma:
         _check(_fn("tree_attention", "zai_tree_attention_mma")(
             out.data_ptr(), qp, qs, kp, ks, vp, vs, pp, bt.data_ptr(), bt.shape[1], cu_q.data_ptr(), ctx_lens.data_ptr(), positions.data_ptr(),
