@@ -145,3 +145,18 @@ def test_sizes_beyond_32_bits_keep_their_meaning():
         with pytest.raises(o.KernelError):
             o.step_layout(**{**dict(q_lens=one, ctx_lens=one, slots=one, page_rows=rows, page_size=4, n_rows=1, width=2), **kw})
     assert o.read_status() == 0
+
+
+def test_the_largest_trees_of_the_tcgen05_kernel():
+    """As many rows as the kernel says it takes, and one more: that goes to another kernel, or is refused."""
+    o = ops()
+    most = o._tree_kernel_takes("tc_rows")
+    for n in (most, most + 1):
+        q, k, v, step, cache, _ = make_tree_step([n, 2], [5000, 40], 4, 2, 64, 64, BF16, 9)
+        close(o.tree_attention(q, k, v, step, cache, 4, 2, 64, 0.125), q, k, v, step, cache, 4, 2, 64, 0.125, None)
+        if n == most:
+            close(o.tree_attention(q, k, v, step, cache, 4, 2, 64, 0.125, impl="tcgen05"), q, k, v, step, cache, 4, 2, 64, 0.125, None)
+            continue
+        with pytest.raises(o.KernelError, match="128 rows"):
+            o.tree_attention(q, k, v, step, cache, 4, 2, 64, 0.125, impl="tcgen05")
+    assert o.read_status() == 0

@@ -1410,7 +1410,7 @@ def step_layout(q_lens, ctx_lens, slots, page_rows, page_size, n_rows, width, pa
 @functools.lru_cache(maxsize=None)
 def _tree_kernel_takes(fn, *sizes):
     """What a tree-attention kernel says of these sizes (asked once: 1.2 us a question)."""
-    return _fn("tree_attention" if fn != "tc_supports" else "tree_attention_tc", "zai_tree_attention_" + fn)(*sizes)
+    return _fn("tree_attention_tc" if fn.startswith("tc_") else "tree_attention", "zai_tree_attention_" + fn)(*sizes)
 
 
 @_timed("attention")
@@ -1461,7 +1461,7 @@ def tree_attention(q, k, v, step, cache, heads, kv_heads, head_dim, scale, windo
     # of 36 behind 300 33 and 40; 8 of 64 behind 1000 21 and 19; 16 of 32 behind 1000 20 and 23; 8 of 32 behind 8000 43 and 36; one of 16
     # behind 30 000 36 and 24; 32 of 16 behind 4000 61 and 62, with heads of 128 102 and 93; one of 256 behind 30 000, heads of 128, 268 and 52)
     long = width >= (256 if most * group > 64 else 1024 if most * group > 32 else 4096)
-    tc = (mma and impl != "mma" and window is None and most <= 128 and (impl == "tcgen05" or long)
+    tc = (mma and impl != "mma" and window is None and (impl == "tcgen05" or long) and most <= _tree_kernel_takes("tc_rows")
           and not (qp & 15 or qs & 7) and _tree_kernel_takes("tc_supports", D, cache.page_size, pages.shape[0], G))
     if impl == "tcgen05" and not tc:
         raise KernelError("tree_attention: the tcgen05 kernel takes bfloat16 heads of 64 or 128 on 16-byte boundaries, trees of at most 128 rows, no window")
