@@ -77,46 +77,22 @@ struct AtArgs {
     ZaiScoreOptions opt;        // (shaped scores)
 };
 
-// two 32-bit numbers in one instruction
-__device__ __forceinline__ float2 at_fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(d))
-        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)), "l"(reinterpret_cast<unsigned long long&>(c)));
-    return d;
-}
-__device__ __forceinline__ float2 at_mul2(float2 a, float2 b) {
-    float2 d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d))
-        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
-    return d;
-}
-__device__ __forceinline__ float2 at_add2(float2 a, float2 b) {
-    float2 d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d))
-        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
-    return d;
-}
 __device__ __forceinline__ uint32_t at_pack(float2 v) {
     __nv_bfloat162 p = __floats2bfloat162_rn(v.x, v.y);
     return *reinterpret_cast<uint32_t*>(&p);
 }
 __device__ __forceinline__ float2 at_two(float v) { return make_float2(v, v); }
-__device__ __forceinline__ float at_max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
 // tanh of two numbers without a branch, so that a warp of mixed scores takes one way: the Taylor series up to x^9 below 0.3 (the next
 // term is under 6e-8 of it there), the identity 1 - 2 / (1 + e^2x) beyond (a relative error of 4e-7 at most).
 __device__ __forceinline__ float2 at_tanh2(float2 x) {
-    const float2 q = at_mul2(x, x);
-    float2 small = at_fma2(q, at_two(62.f / 2835.f), at_two(-17.f / 315.f));
-    small = at_fma2(q, small, at_two(2.f / 15.f));
-    small = at_fma2(q, small, at_two(-1.f / 3.f));
-    small = at_fma2(at_mul2(x, q), small, x);
-    const float2 z = at_mul2(x, at_two(2.8853900817779268f));
-    const float2 d = at_add2(make_float2(at_exp2(z.x), at_exp2(z.y)), at_two(1.f));
-    const float2 large = at_fma2(make_float2(__fdividef(1.f, d.x), __fdividef(1.f, d.y)), at_two(-2.f), at_two(1.f));
+    const float2 q = zai_mul2(x, x);
+    float2 small = zai_fma2(q, at_two(62.f / 2835.f), at_two(-17.f / 315.f));
+    small = zai_fma2(q, small, at_two(2.f / 15.f));
+    small = zai_fma2(q, small, at_two(-1.f / 3.f));
+    small = zai_fma2(zai_mul2(x, q), small, x);
+    const float2 z = zai_mul2(x, at_two(2.8853900817779268f));
+    const float2 d = zai_add2(make_float2(at_exp2(z.x), at_exp2(z.y)), at_two(1.f));
+    const float2 large = zai_fma2(make_float2(__fdividef(1.f, d.x), __fdividef(1.f, d.y)), at_two(-2.f), at_two(1.f));
     return make_float2(fabsf(x.x) < 0.3f ? small.x : large.x, fabsf(x.y) < 0.3f ? small.y : large.y);
 }
 
@@ -449,7 +425,7 @@ __global__ void __launch_bounds__(AT_THREADS, 2) prefill_tc_kernel(const __grid_
                         for (int j = 0; j < KEYS; j += 2) {
                             float2 v = make_float2(__uint_as_float(x[j >> 5][j & 31]), __uint_as_float(x[j >> 5][(j & 31) + 1]));
                             const float2 add = make_float2(entry(j), entry(j + 1));
-                            v = a.opt.softcap > 0.f ? at_fma2(at_tanh2(at_mul2(v, at_two(unit))), at_two(cap), add) : at_fma2(v, at_two(a.scale_log2), add);
+                            v = a.opt.softcap > 0.f ? zai_fma2(at_tanh2(zai_mul2(v, at_two(unit))), at_two(cap), add) : zai_fma2(v, at_two(a.scale_log2), add);
                             x[j >> 5][j & 31] = __float_as_uint(v.x);
                             x[j >> 5][(j & 31) + 1] = __float_as_uint(v.y);
                         }
@@ -472,8 +448,8 @@ __global__ void __launch_bounds__(AT_THREADS, 2) prefill_tc_kernel(const __grid_
                 float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};            // four chains, not one of 32 links
 #pragma unroll
                 for (int j = 0; j < KEYS; j += 2)
-                    mx4[(j >> 1) & 3] = at_max3(mx4[(j >> 1) & 3], __uint_as_float(x[j >> 5][j & 31]), __uint_as_float(x[j >> 5][(j & 31) + 1]));
-                const float mx = fmaxf(at_max3(mx4[0], mx4[1], mx4[2]), mx4[3]) * c;
+                    mx4[(j >> 1) & 3] = zai_max3(mx4[(j >> 1) & 3], __uint_as_float(x[j >> 5][j & 31]), __uint_as_float(x[j >> 5][(j & 31) + 1]));
+                const float mx = fmaxf(zai_max3(mx4[0], mx4[1], mx4[2]), mx4[3]) * c;
                 // move the reference?  (warp-wide decision: the TMEM accesses below are the whole warp's)
                 float alpha = 1.f, ref = m;
                 if (!SHAPED && i > 0) {
@@ -515,14 +491,14 @@ __global__ void __launch_bounds__(AT_THREADS, 2) prefill_tc_kernel(const __grid_
                     uint32_t pk[8];
 #pragma unroll
                     for (int j = j0; j < j0 + 16; j += 2) {
-                        const float2 z = at_fma2(make_float2(__uint_as_float(x[j >> 5][j & 31]), __uint_as_float(x[j >> 5][(j & 31) + 1])), c2, minus);
+                        const float2 z = zai_fma2(make_float2(__uint_as_float(x[j >> 5][j & 31]), __uint_as_float(x[j >> 5][(j & 31) + 1])), c2, minus);
                         const float2 p = make_float2(at_exp2(z.x), at_exp2(z.y));
-                        lt[(j >> 1) & 3] = at_add2(lt[(j >> 1) & 3], p);
+                        lt[(j >> 1) & 3] = zai_add2(lt[(j >> 1) & 3], p);
                         pk[(j - j0) >> 1] = at_pack(p);
                     }
                     at_tmem_st8(tP + j0 / 2, pk);
                 }
-                const float2 sum = at_add2(at_add2(lt[0], lt[1]), at_add2(lt[2], lt[3]));
+                const float2 sum = zai_add2(zai_add2(lt[0], lt[1]), zai_add2(lt[2], lt[3]));
                 l += sum.x + sum.y;
                 // P (and a rescaled O) are in TMEM before the product-issuing thread hears of it
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");

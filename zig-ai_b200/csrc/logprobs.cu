@@ -64,29 +64,6 @@ __device__ __forceinline__ Sums joined(const Sums& a, const Sums& b) {
     return r;
 }
 
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d))
-        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
-    return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d))
-        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
-    return d;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(d))
-        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)), "l"(reinterpret_cast<unsigned long long&>(c)));
-    return d;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
 __device__ __forceinline__ float pow2_of(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -207,8 +184,8 @@ __global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_kernel(float* __
     auto round = [&](const float (&x)[LP_ROUND], int at) {
         float top4[LP_ROUND / 4], top_x;
 #pragma unroll
-        for (int e = 0; e < LP_ROUND; e += 4) top4[e / 4] = fmaxf(max3(x[e], x[e + 1], x[e + 2]), x[e + 3]);
-        top_x = fmaxf(max3(top4[0], top4[1], top4[2]), top4[3]);
+        for (int e = 0; e < LP_ROUND; e += 4) top4[e / 4] = fmaxf(zai_max3(x[e], x[e + 1], x[e + 2]), x[e + 3]);
+        top_x = fmaxf(zai_max3(top4[0], top4[1], top4[2]), top4[3]);
         if (TOP) {
             // (the entries of the lanes that have such a key are looked at once more, in memory, by few instructions: with the registers' sixteen
             // copies of this code it was a third of the kernel, most of it their own arrival)
@@ -243,9 +220,9 @@ __global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_kernel(float* __
             const float2 m2 = make_float2(-mine.m, -mine.m), l2 = make_float2(1.4426950408889634f, 1.4426950408889634f);
 #pragma unroll
             for (int e = 0; e < LP_ROUND; e += 2) {
-                const float2 d = add2(make_float2(x[e], x[e + 1]), m2), p = mul2(d, l2), w = make_float2(pow2_of(p.x), pow2_of(p.y));
-                z = add2(z, w);
-                u = fma2(w, d, u);
+                const float2 d = zai_add2(make_float2(x[e], x[e + 1]), m2), p = zai_mul2(d, l2), w = make_float2(pow2_of(p.x), pow2_of(p.y));
+                z = zai_add2(z, w);
+                u = zai_fma2(w, d, u);
             }
             if (u.x != u.x || u.y != u.y) {                    // 0 times -inf, which is 0 here
                 u = make_float2(0.f, 0.f);

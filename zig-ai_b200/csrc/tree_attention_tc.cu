@@ -243,24 +243,6 @@ __device__ __forceinline__ void begin_walk(const TtArgs& a, int D, long long* sh
 // each), while the other waits, loads and compares: 67 instead of 71 us for the 32 trees above, 58 instead of 61 for 8 of 33-64 rows.
 #define TT_SYNC(i) asm volatile("bar.sync %0, 64;" ::"r"(2 + (i)) : "memory")
 #define TT_ARRIVE(i) asm volatile("bar.arrive %0, 64;" ::"r"(2 + (i)) : "memory")
-// two 32-bit numbers in one instruction
-__device__ __forceinline__ float2 tt_fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(d))
-        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)), "l"(reinterpret_cast<unsigned long long&>(c)));
-    return d;
-}
-__device__ __forceinline__ float2 tt_add2(float2 a, float2 b) {
-    float2 d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d))
-        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
-    return d;
-}
-__device__ __forceinline__ float tt_max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
 __device__ __forceinline__ void tt_ld16_nowait(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
@@ -662,11 +644,11 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attention_tc_kernel(const 
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int j = 0; j < 32; j += 2)
-                        mx[(j >> 1) & 7] = tt_max3(mx[(j >> 1) & 7], __uint_as_float(x[i][j]), __uint_as_float(x[i][j + 1]));
+                        mx[(j >> 1) & 7] = zai_max3(mx[(j >> 1) & 7], __uint_as_float(x[i][j]), __uint_as_float(x[i][j + 1]));
                 // The reference is the first tile's maximum, and moves when a later one exceeds it by 2^8: a weight keeps its 8 bits whatever the
                 // reference is.  They are rounded for the product, their sum is taken before, in 32 bits (the sum of the rounded ones would
                 // make one key alone exact, and costs two instructions more a key: 66 instead of 63 us for 32 trees).
-                const float most = tt_max3(tt_max3(mx[0], mx[1], mx[2]), tt_max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * c;
+                const float most = zai_max3(zai_max3(mx[0], mx[1], mx[2]), zai_max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * c;
                 const float top = !begun || m == -INFINITY ? most : most > m + 8.f ? most : m;
                 if (begun && __any_sync(0xffffffffu, top != m)) {
                     // O with the turn's last product in it (those before it came ahead of these scores)
@@ -693,9 +675,9 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attention_tc_kernel(const 
                 uint32_t pk[32];
 #pragma unroll
                 for (int j = 0; j < 64; j += 2) {
-                    const float2 e = tt_fma2(make_float2(__uint_as_float(x[j >> 5][j & 31]), __uint_as_float(x[j >> 5][(j & 31) + 1])), c2, minus);
+                    const float2 e = zai_fma2(make_float2(__uint_as_float(x[j >> 5][j & 31]), __uint_as_float(x[j >> 5][(j & 31) + 1])), c2, minus);
                     const float2 w2 = make_float2(at_exp2(e.x), at_exp2(e.y));
-                    sums[(j >> 1) & 1] = tt_add2(sums[(j >> 1) & 1], w2);
+                    sums[(j >> 1) & 1] = zai_add2(sums[(j >> 1) & 1], w2);
                     pk[j >> 1] = pack_bf16(w2.x, w2.y);
                 }
                 at_tmem_st32(tB, pk);
@@ -703,7 +685,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attention_tc_kernel(const 
                     --left;
                     if (turn == 0 || left > 0) TT_ARRIVE((turn ^ 1) * 4 + qd);
                 }
-                const float2 sum = tt_add2(sums[0], sums[1]);
+                const float2 sum = zai_add2(sums[0], sums[1]);
                 l += sum.x + sum.y;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
