@@ -13,9 +13,11 @@
 // so that as many rounds again note as many again.  A key's place is the number of noted keys above it.  A row that
 // notes more than there is room for (one that ascends) is walked again in steps that cut the list down as they go.
 //
-// What bounds it: the instructions, six to seven an entry (a load's quarter, half a maximum, half each of the difference, the product with log2 e and the
-// two sums, which take two numbers at a time, the exponential, and two for the rank), so that is what they are kept to: a thread looks for
-// keys to note only where its round's maximum reaches the bound, and 0 times -inf, which only masked tokens bring, is put right afterwards.
+// What bounds it: instructions and the wait for memory together.  An entry takes 13 instructions of a thread without alternatives, 16 with five
+// and 22 with 32, in either type (counted over 2048 rows of 64 401 and 65 536); they fill 56 to 60 % of the issue slots.  What a warp waits for
+// between two of them is its next round's loads (half of the wait without alternatives; with five a fifth, and as much for the barriers of
+// the list's cuts).  bfloat16 rows are half the bytes and the same instructions, and take as long.  So a thread looks for keys to note only where its
+// round's maximum reaches the bound, the sums take two numbers an instruction, and 0 times -inf, which only masked tokens bring, is put right afterwards.
 //
 // A row is split over a cluster of up to 16 blocks when there are few rows; the first block joins the parts through distributed shared memory.
 // Measured: 2048 rows of 64 401 in 32 bits 87 us without alternatives (6.1 TB/s), 103 with 5, 121 with 20, 139 with 32; in
@@ -57,7 +59,7 @@ __device__ __forceinline__ Sums joined(const Sums& a, const Sums& b) {
         r.u += f * (a.u + d * a.z);
     }
     if (b.m != -INFINITY) {
-        const float d = fmaxf(b.m - m, -150.f), f = exp_of(d);     // (0 beyond that, which a difference near the type's end must not turn into NaN)
+        const float d = fmaxf(b.m - m, -150.f), f = exp_of(d);
         r.z += f * b.z;
         r.u += f * (b.u + d * b.z);
     }

@@ -375,10 +375,11 @@ __global__ void __launch_bounds__(GEN_THREADS) tree_attention_general_kernel(con
 // ---------------------------------------------------------------------------------------------------- bfloat16 on mma.sync
 // A block owns 16 WM pairs; its warps are WM rows of 16 pairs times WN shares of every tile of KEYS keys, each share with a maximum,
 // a sum and an O of its own (joined with those of the cluster's other blocks at the end).  Keys and values come by cp.async, STAGES tiles
-// in a ring; where a tile's 64 keys lie is looked up a turn before its copies are issued, by one thread a key.  Q stays in registers,
-// scores go from the accumulators into the second product's operand without leaving them.  Weights are rounded to bfloat16 there, as
-// the values are; their sum is taken before the rounding, in 32 bits.  Shared memory decides how many blocks an SM holds: a tile's places
-// take two entries, not four, because with four the second block did not fit (22 instead of 12 us for the tree above).
+// in a ring; where a tile's keys (64, or 128 where a block has up to 32 pairs of heads of up to 64) lie is looked up a turn before its copies
+// are issued, by one thread a key.  Q stays in registers, scores go from the accumulators into the second product's operand without leaving
+// them.  Weights are rounded to bfloat16 there, as the values are; their sum is taken before the rounding, in 32 bits.  Shared memory decides
+// how many blocks an SM holds: a tile's places take two entries, not four, because with four the second block did not fit (22 instead of
+// 12 us for the tree above).
 
 template <int D, int WM, int WN, int KEYS, int STAGES> struct MmaShape {
     static_assert(KEYS <= 32 * WM * WN && KEYS / WN % 16 == 0, "a thread a key looks up where it lies");

@@ -54,8 +54,10 @@ struct TtArgs {
 };
 
 // ---- the list of tiles.  A request with n rows has units of 256 pairs by key/value head, the last ones of what is left; each unit has a
-// tile for every 128 cached keys and one for the drafted rows.  With heads of 64 a tile that both turns work on costs twice what one of
-// a turn alone does; with heads of 128, where the ring holds two tiles and a turn alone waits for the next, they cost the same.
+// tile for every 64 cached keys and one or two for the drafted rows.  What a tile that both turns work on costs beside one of a turn alone: with
+// heads of 64 twice as much (the softmax's chain is the limit; counted the same, 32 trees of 4-24 rows take as long, 70 us with L2 flushed, and 8 of
+// 33-64 rows 92 instead of 94); with heads of 128 the same (8 trees of 24-64 rows behind 4000-30000 positions 156 us, counted double 168; one of 64
+// behind 30 000 63.5 and 65.7).
 struct Request { int first, n, ctx, cached, tiles, row_units, last_cost; };
 __device__ __forceinline__ int unit_cost(const TtArgs& a, int pairs) { return pairs > TT_TILE ? a.dual_cost : 1; }
 __device__ __forceinline__ Request request_of(const TtArgs& a, int s, bool say) {
@@ -646,8 +648,9 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attention_tc_kernel(const 
                     for (int j = 0; j < 32; j += 2)
                         mx[(j >> 1) & 7] = zai_max3(mx[(j >> 1) & 7], __uint_as_float(x[i][j]), __uint_as_float(x[i][j + 1]));
                 // The reference is the first tile's maximum, and moves when a later one exceeds it by 2^8: a weight keeps its 8 bits whatever the
-                // reference is.  They are rounded for the product, their sum is taken before, in 32 bits (the sum of the rounded ones would
-                // make one key alone exact, and costs two instructions more a key: 66 instead of 63 us for 32 trees).
+                // reference is.  They are rounded for the product, their sum is taken before, in 32 bits.  (The rounded ones' sum: 2.17e-3 instead
+                // of 2.27e-3 from 64 bits for 32 trees, root mean square, and 2 to 6 us more; the rest is the rounding of the weights themselves and
+                // of the result, 1.66e-3 together where the products are made in 32 bits.)
                 const float most = zai_max3(zai_max3(mx[0], mx[1], mx[2]), zai_max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * c;
                 const float top = !begun || m == -INFINITY ? most : most > m + 8.f ? most : m;
                 if (begun && __any_sync(0xffffffffu, top != m)) {
