@@ -11,7 +11,7 @@
 //                           mask[r]   = bits of r's ancestors and of r among the span's rows
 //                       and one more span, of no request, for the rows behind the last one
 //   zai_accept_drafts   cur = 0; while some child c of cur has token[c] == choice[cur]: cur = the first such c
-//   zai_commit_drafts   keys and values of the accepted rows into the pages, in all layers of a cache group at once
+//   zai_commit_drafts   keys and values of the accepted rows into the pages, of one layer (as ModelRunner.verify calls it) or of several at once
 //
 // All three are a few kilobytes of whole numbers (the last a few megabytes): what bounds them is a launch and two or three trips to
 // memory that depend on one another, so each is one kernel, blocks need nothing of one another, and what a block would need from
